@@ -211,6 +211,97 @@ int tg_int8_gemv_dequant(const int8_t *xq, const float *xscale, const int8_t *wq
  */
 int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
 
+/* Most activation rows tg_int4_gemv_dequant accepts. */
+#define TG_INT4_MAX_M 64
+
+/*
+ * Few activation rows (1 <= M <= TG_INT4_MAX_M) times a weight held in 4 bits
+ * with one scale for each group of input channels: half the weight bytes of
+ * tg_int8_gemv_dequant, for linears that are bound by them.  The activations
+ * are the quantiser's codes and scales (tg_rotate_quant, tg_quantize_act,
+ * tg_quantize_ln_mod).  No reference counterpart (its weights are int8).
+ *
+ *   out[m,n] = (sum_g wscale[n,g] * float(sum_{k in g} xq[m,k] * w4[n,k])) * xscale[m] + bias[n]
+ *
+ * The inner sums are exact, the outer one is fp32, in an order that depends on
+ * N and K only (a row's result does not depend on the other rows or on M).
+ *
+ *   xq      [M, K] int8, 16-B aligned; K % 128 == 0
+ *   w4      [N, K/2] bytes, 16-B aligned: of each 128 codes of a row, byte
+ *           16 t + 4 j + b (t, j, b = 0..3) holds code 32 j + 8 t + b in its low
+ *           and code 32 j + 8 t + 4 + b in its high half, two's complement
+ *   wscale  [N, K/group] of wscale_dtype (TG_DT_F32/F16/BF16)
+ *   group   32, 64, 128 or 256 consecutive codes; K % group == 0
+ *   bias    [N] of bias_dtype or NULL; out [M, N] of out_dtype (any N)
+ * M == 0 is a no-op; TG_ERR_UNSUPPORTED for M > TG_INT4_MAX_M.
+ */
+int tg_int4_gemv_dequant(const int8_t *xq, const float *xscale, const uint8_t *w4, const void *wscale,
+                         int wscale_dtype, int group, const void *bias, int bias_dtype, int64_t M, int64_t N,
+                         int64_t K, int out_dtype, void *out, void *stream);
+
+/*
+ * The router of a layer with routed experts: each token's top_k experts, their
+ * weights, and the (token, expert) slots sorted by expert, all on the device.
+ * No reference counterpart, nor have the three functions below.
+ *
+ *   logits   [T, E] of dtype (TG_DT_F32/F16/BF16); E <= TG_MAX_EXPERTS,
+ *            top_k <= min(E, TG_MAX_TOP_K)
+ *   ids      [T, top_k] out: the experts of the largest logits, descending;
+ *            equal logits by ascending index, NaN above everything
+ *   weights  [T, top_k] fp32 out: exp(l - l_max) / sum, the sum over the
+ *            chosen experts (renormalize != 0) or over all E
+ *   offsets  [E + 1] out: expert e's rows are offsets[e] .. offsets[e+1] - 1
+ *   rows     [T * top_k] out: row r's token; the rows behind offsets[E]: -1
+ *   place    [T, top_k] out: the row of slot (t, j)
+ * Rows are in order of (expert, token).  A slot whose logit is -inf (a closed
+ * expert, a padded token) is left out: id and place -1, weight 0.
+ * `workspace`: tg_route_experts_workspace(T, E) bytes, 4-byte aligned; needs no
+ * initial value and holds nothing between calls.  T == 0 writes zero offsets.
+ */
+#define TG_MAX_EXPERTS 1024
+#define TG_MAX_TOP_K 32
+int tg_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int top_k, int renormalize,
+                     float *weights, int32_t *ids, int32_t *offsets, int32_t *rows, int32_t *place, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Workspace bytes of tg_route_experts. */
+size_t tg_route_experts_workspace(int64_t T, int64_t E);
+
+/*
+ * tg_int8_gemm_dequant with one weight per expert over ragged groups of rows:
+ * for e < E and offsets[e] <= r < offsets[e+1], with a = rows[r] (or r where
+ * rows is NULL),
+ *   out[r,n] = ((float(sum_k xq[a,k] * wq[e,n,k]) * xscale[a]) * wscale[e,n]) + bias[e,n]
+ * each row bit-identical to tg_int8_gemm_dequant with that expert's weight.
+ *
+ *   xq       [M, K] int8, xscale [M]; K % 16 == 0
+ *   wq       [E, N, K] int8; wscale fp32 of 1, E or E*N elements
+ *   bias     [E, N] of bias_dtype or NULL
+ *   rows     [R] row of xq behind each output row, or NULL (then R <= M); an
+ *            index outside [0, M) stands for a row of zeros
+ *   offsets  [E + 1] ascending, on the device; read as min(max(., 0), R)
+ *   out      [R, N] of out_dtype; N*sizeof(out) % 16 == 0; rows that no group
+ *            covers are left as they were
+ * xq, wq and out 16-B aligned; E <= TG_MAX_EXPERTS.  R == 0 is a no-op.
+ */
+int tg_int8_grouped_gemm_dequant(const int8_t *xq, const float *xscale, int64_t M, const int8_t *wq,
+                                 const float *wscale, int64_t wscale_numel, const void *bias, int bias_dtype,
+                                 const int32_t *rows, const int32_t *offsets, int64_t R, int64_t E, int64_t N,
+                                 int64_t K, int out_dtype, void *out, void *stream);
+
+/*
+ * Each token's experts' rows added up:
+ *   out[t,:] = sum_j weights[t,j] * y[place[t,j],:] (+ residual[t,:])
+ * in fp32, j ascending, then the residual, rounded once.
+ *
+ *   y        [R, N] of dtype; place [T, top_k], a place outside [0, R) adds
+ *            nothing; weights [T, top_k] fp32; residual [T, N] of dtype or NULL
+ *   out      [T, N] of dtype (may be `residual` itself)
+ * Any N; top_k <= TG_MAX_TOP_K.  T == 0 is a no-op.
+ */
+int tg_combine_experts(const void *y, int dtype, int64_t R, const int32_t *place, const float *weights, int64_t T,
+                       int top_k, const void *residual, int64_t N, void *out, void *stream);
+
 /*
  * tg_int8_gemm_dequant_splitk for callers that cannot allocate device memory:
  * a plugin running inside a host application that owns all GPU memory through

@@ -1,0 +1,191 @@
+"""4-bit weights and routed experts without a GPU: the packed layout, the weight quantiser, and every
+argument check that returns before device work (Python and C ABI)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from tilegen_b200 import _lib, ops
+from tilegen_b200.quant import (int4_linear, int8_expert_ffn, pack_int4, quantize_convrot_expert_weights,
+                                quantize_convrot_weight, quantize_convrot_weight_int4, unpack_int4)
+
+P = ctypes.c_void_p(256)
+OK, ARG, UNS, MIS = _lib.TG_OK, _lib.TG_ERR_INVALID_ARG, _lib.TG_ERR_UNSUPPORTED, _lib.TG_ERR_MISALIGNED
+
+
+# ---------------------------------------------------------------- layout and weight quantiser
+@pytest.mark.parametrize("n,k", [(1, 128), (3, 256), (16, 640), (0, 128)])
+def test_pack_roundtrip_and_layout(n, k):
+    codes = torch.randint(-8, 8, (n, k), generator=torch.Generator().manual_seed(k), dtype=torch.int8)
+    w4 = pack_int4(codes)
+    assert w4.shape == (n, k // 2) and w4.dtype == torch.uint8
+    assert torch.equal(unpack_int4(w4), codes)
+    for row in range(n):
+        for block in range(k // 128):
+            for byte in (0, 3, 4, 17, 42, 63):
+                t, j, b = byte // 16, byte % 16 // 4, byte % 4
+                at = block * 128 + 32 * j + 8 * t + b
+                v = int(w4[row, block * 64 + byte])
+                assert v & 15 == int(codes[row, at]) & 15 and v >> 4 == int(codes[row, at + 4]) & 15
+
+
+def test_pack_refusals():
+    for bad in (torch.zeros(4, 120, dtype=torch.int8), torch.zeros(128, dtype=torch.int8), torch.zeros(4, 128)):
+        with pytest.raises(ValueError):
+            pack_int4(bad)
+    for v in (-9, 8):
+        with pytest.raises(ValueError, match="outside"):
+            pack_int4(torch.full((1, 128), v, dtype=torch.int8))
+    for bad in (torch.zeros(4, 60, dtype=torch.uint8), torch.zeros(4, 64, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            unpack_int4(bad)
+
+
+@pytest.mark.parametrize("scale_group", [32, 64, 128, 256])
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_weight_quantiser_error(scale_group, scale_dtype):
+    """Each rotated value is within half a step of its code times the stored scale; at the clip (a scale
+    rounded down) by at most 7 times the scale's own rounding more."""
+    from tilegen_b200.kernels.hadamard import build_hadamard, rotate_by_group
+
+    w = torch.randn(24, 512, generator=torch.Generator().manual_seed(1))
+    w[3] = 0
+    w4, ws = quantize_convrot_weight_int4(w, 256, scale_group, scale_dtype)
+    assert ws.dtype == scale_dtype and ws.shape == (24, 512 // scale_group)
+    rot = rotate_by_group(w.double(), build_hadamard(256, "cpu", torch.float64), 256).view(24, -1, scale_group)
+    got = unpack_int4(w4).double().view(24, -1, scale_group) * ws.double()[..., None]
+    step = ws.double()[..., None]
+    slack = 7 * step * torch.finfo(scale_dtype).eps / 2 + 1e-5  # + the rotation in fp32
+    assert ((got - rot).abs() <= step / 2 + slack).all()
+    assert (got[3] == 0).all()
+
+
+def test_weight_quantiser_refusals():
+    w = torch.zeros(4, 256)
+    for kwargs in ({"scale_group": 16}, {"scale_group": 512}, {"scale_dtype": torch.float64}, {"group_size": 512}):
+        with pytest.raises(ValueError):
+            quantize_convrot_weight_int4(w, **kwargs)
+    with pytest.raises(ValueError):
+        quantize_convrot_weight_int4(torch.zeros(4, 2, 256))
+    with pytest.raises(ValueError):
+        quantize_convrot_weight_int4(torch.zeros(4, 64), scale_group=64)
+    for v in (float("nan"), float("inf"), 1e9):
+        w[1, 3] = v
+        with pytest.raises(ValueError, match="cannot hold"):
+            quantize_convrot_weight_int4(w)
+
+
+def test_expert_weights_are_each_experts_weight():
+    w = torch.randn(3, 16, 256, generator=torch.Generator().manual_seed(2))
+    wq, ws = quantize_convrot_expert_weights(w)
+    for e in range(3):
+        q, s = quantize_convrot_weight(w[e])
+        assert torch.equal(wq[e], q) and torch.equal(ws[e], s)
+    with pytest.raises(ValueError):
+        quantize_convrot_expert_weights(w[0])
+
+
+# ---------------------------------------------------------------- Python refusals
+def test_cpu_tensors_are_refused():
+    i8, f = torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.int4_gemv_dequant(i8, f, torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 1), None, torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.route_experts(torch.zeros(2, 4), 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.int8_grouped_gemm_dequant(i8, f, torch.zeros(2, 8, 128, dtype=torch.int8), f, None,
+                                      torch.zeros(3, dtype=torch.int32), torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.combine_experts(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
+
+
+def test_layer_functions_check_shapes():
+    with pytest.raises(ValueError, match="differ"):
+        int4_linear(torch.zeros(2, 256), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 1))
+    up = (torch.zeros(2, 512, 256, dtype=torch.int8), torch.zeros(2, 512), None)
+    down = (torch.zeros(2, 256, 512, dtype=torch.int8), torch.zeros(2, 256), None)
+    with pytest.raises(ValueError, match="logits"):
+        int8_expert_ffn(torch.zeros(3, 256), torch.zeros(2, 2), up, down, 1)
+    with pytest.raises(ValueError, match="channels"):
+        int8_expert_ffn(torch.zeros(3, 256), torch.zeros(3, 2), up, up, 1)
+
+
+def test_custom_ops_trace_on_meta():
+    m = torch.device("meta")
+    y = torch.ops.tilegen.int4_gemv_dequant(torch.empty(3, 256, dtype=torch.int8, device=m), torch.empty(3, device=m),
+                                            torch.empty(7, 128, dtype=torch.uint8, device=m),
+                                            torch.empty(7, 2, device=m), None, torch.bfloat16)
+    assert y.shape == (3, 7) and y.dtype == torch.bfloat16
+    w, ids, offsets, rows, place = torch.ops.tilegen.route_experts(torch.empty(5, 8, device=m), 2, True)
+    assert (w.shape, ids.shape, offsets.shape, rows.shape, place.shape) == ((5, 2), (5, 2), (9,), (10,), (5, 2))
+    xq, wq = torch.empty(5, 64, dtype=torch.int8, device=m), torch.empty(8, 24, 64, dtype=torch.int8, device=m)
+    y = torch.ops.tilegen.int8_grouped_gemm_dequant(xq, torch.empty(5, device=m), wq, torch.empty(8, 24, device=m), None,
+                                                    offsets, torch.float16, rows)
+    assert y.shape == (10, 24) and y.dtype == torch.float16
+    assert torch.ops.tilegen.combine_experts(y, place, w, None).shape == (5, 24)
+
+
+# ---------------------------------------------------------------- C ABI refusals
+def _int4(xq=P, xs=P, w4=P, ws=P, wdt=1, group=128, bias=None, bdt=0, m=1, n=16, k=256, odt=1, out=P):
+    return _lib.lib().tg_int4_gemv_dequant(xq, xs, w4, ws, wdt, group, bias, bdt, m, n, k, odt, out, None)
+
+
+@pytest.mark.parametrize("kwargs,status", [
+    ({"m": -1}, ARG), ({"n": 0}, ARG), ({"k": 0}, ARG), ({"odt": 3}, ARG), ({"wdt": 9}, ARG),
+    ({"bias": P, "bdt": 5}, ARG), ({"group": 16}, UNS), ({"group": 512}, UNS), ({"m": 65}, UNS), ({"k": 192}, UNS),
+    ({"k": 384, "group": 256}, UNS), ({"xq": None}, ARG), ({"xs": None}, ARG), ({"w4": None}, ARG), ({"ws": None}, ARG),
+    ({"out": None}, ARG), ({"w4": ctypes.c_void_p(264)}, MIS), ({"xq": ctypes.c_void_p(8)}, MIS),
+    ({"out": ctypes.c_void_p(257)}, MIS), ({"ws": ctypes.c_void_p(257)}, MIS), ({"m": 0, "xq": None, "out": None}, OK),
+    ({"n": 1 << 31}, UNS),
+])
+def test_int4_entry_checks(kwargs, status):
+    assert _int4(**kwargs) == status
+
+
+def _route(logits=P, dt=0, t=4, e=8, k=2, w=P, ids=P, offsets=P, rows=P, place=P, ws=P, bytes=1 << 20):
+    return _lib.lib().tg_route_experts(logits, dt, t, e, k, 1, w, ids, offsets, rows, place, ws, bytes, None)
+
+
+@pytest.mark.parametrize("kwargs,status", [
+    ({"t": -1}, ARG), ({"e": 0}, ARG), ({"k": 0}, ARG), ({"k": 9}, ARG), ({"dt": 4}, ARG), ({"e": 1025}, UNS),
+    ({"e": 64, "k": 33}, UNS), ({"t": 1 << 30}, UNS), ({"offsets": None}, ARG), ({"logits": None}, ARG), ({"w": None}, ARG),
+    ({"ids": None}, ARG), ({"rows": None}, ARG), ({"place": None}, ARG), ({"ws": None}, ARG), ({"bytes": 31}, ARG),
+    ({"logits": ctypes.c_void_p(258)}, MIS), ({"place": ctypes.c_void_p(258)}, MIS), ({"offsets": ctypes.c_void_p(258)}, MIS),
+])
+def test_route_entry_checks(kwargs, status):
+    assert _lib.lib().tg_route_experts_workspace(4, 8) >= 32
+    assert _lib.lib().tg_route_experts_workspace(0, 8) == 0
+    assert _route(**kwargs) == status
+
+
+def _grouped(xq=P, xs=P, m=4, wq=P, ws=P, wn=1, bias=None, bdt=0, rows=P, offsets=P, r=8, e=2, n=64, k=64, odt=1, out=P):
+    return _lib.lib().tg_int8_grouped_gemm_dequant(xq, xs, m, wq, ws, wn, bias, bdt, rows, offsets, r, e, n, k, odt, out,
+                                                   None)
+
+
+@pytest.mark.parametrize("kwargs,status", [
+    ({"m": -1}, ARG), ({"r": -1}, ARG), ({"e": 0}, ARG), ({"n": 0}, ARG), ({"k": 0}, ARG), ({"odt": 7}, ARG),
+    ({"bias": P, "bdt": 7}, ARG), ({"wn": 3}, ARG), ({"rows": None}, ARG), ({"k": 24}, UNS), ({"n": 12}, UNS),
+    ({"n": 2, "odt": 0}, UNS), ({"e": 1025}, UNS), ({"e": 1000, "n": 1 << 22}, UNS), ({"xq": None}, ARG), ({"xs": None}, ARG), ({"wq": None}, ARG),
+    ({"ws": None}, ARG), ({"offsets": None}, ARG), ({"out": None}, ARG), ({"xq": ctypes.c_void_p(8)}, MIS),
+    ({"wq": ctypes.c_void_p(8)}, MIS), ({"out": ctypes.c_void_p(8)}, MIS), ({"rows": ctypes.c_void_p(2)}, MIS),
+    ({"r": 0, "out": None}, OK), ({"m": 0, "r": 0, "xq": None}, OK),
+])
+def test_grouped_entry_checks(kwargs, status):
+    assert _grouped(**kwargs) == status
+
+
+def _combine(y=P, dt=1, r=8, place=P, w=P, t=4, k=2, res=None, n=64, out=P):
+    return _lib.lib().tg_combine_experts(y, dt, r, place, w, t, k, res, n, out, None)
+
+
+@pytest.mark.parametrize("kwargs,status", [
+    ({"t": -1}, ARG), ({"r": -1}, ARG), ({"n": 0}, ARG), ({"k": 0}, ARG), ({"dt": 3}, ARG), ({"k": 33}, UNS), ({"t": 1 << 31}, UNS),
+    ({"y": None}, ARG), ({"place": None}, ARG), ({"w": None}, ARG), ({"out": None}, ARG), ({"y": ctypes.c_void_p(257)}, MIS),
+    ({"out": ctypes.c_void_p(257)}, MIS), ({"res": ctypes.c_void_p(257)}, MIS), ({"place": ctypes.c_void_p(2)}, MIS),
+    ({"t": 0, "y": None, "out": None}, OK),
+])
+def test_combine_entry_checks(kwargs, status):
+    assert _combine(**kwargs) == status

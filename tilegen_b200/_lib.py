@@ -125,6 +125,16 @@ def lib() -> ctypes.CDLL:
         L.tg_int8_gemv_dequant.restype = i32
         L.tg_int8_gemv_dequant_config.argtypes = [i64, i64, ctypes.POINTER(i32), ctypes.POINTER(i32)]
         L.tg_int8_gemv_dequant_config.restype = i32
+        L.tg_int4_gemv_dequant.argtypes = [p, p, p, p, i32, i32, p, i32, i64, i64, i64, i32, p, p]
+        L.tg_int4_gemv_dequant.restype = i32
+        L.tg_route_experts.argtypes = [p, i32, i64, i64, i32, i32, p, p, p, p, p, p, ctypes.c_size_t, p]
+        L.tg_route_experts.restype = i32
+        L.tg_route_experts_workspace.argtypes = [i64, i64]
+        L.tg_route_experts_workspace.restype = ctypes.c_size_t
+        L.tg_int8_grouped_gemm_dequant.argtypes = [p, p, i64, p, p, i64, p, i32, p, p, i64, i64, i64, i64, i32, p, p]
+        L.tg_int8_grouped_gemm_dequant.restype = i32
+        L.tg_combine_experts.argtypes = [p, i32, i64, p, p, i64, i32, p, i64, p, p]
+        L.tg_combine_experts.restype = i32
         L.tg_peer_handle_bytes.restype = ctypes.c_size_t
         L.tg_peer_alloc.argtypes = [ctypes.c_size_t, ctypes.POINTER(p), p]
         L.tg_peer_alloc.restype = i32

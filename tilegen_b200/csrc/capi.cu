@@ -7,8 +7,11 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "experts.cuh"
+#include "gemm_grouped.cuh"
 #include "gemm_i8.cuh"
 #include "gemm_splitk.cuh"
+#include "gemv_i4.cuh"
 #include "gemv_i8.cuh"
 #include "rotquant.cuh"
 
@@ -1061,6 +1064,211 @@ int tg_copy_async(void* dst, const void* src, size_t bytes, void* stream) {
                  cudaSuccess
              ? TG_OK
              : TG_ERR_CUDA;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------ 4-bit weights, few rows
+namespace {
+
+bool is_dtype(int d) { return d == TG_DT_F32 || d == TG_DT_F16 || d == TG_DT_BF16; }
+
+size_t dtype_bytes(int d) { return d == TG_DT_F32 ? 4 : 2; }
+
+bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// A launch as the programmatic dependent of the kernel before it.
+template <typename P>
+int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, uint32_t smem, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return TG_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w4, const void* wscale,
+                         int wscale_dtype, int group, const void* bias, int bias_dtype, int64_t M, int64_t N,
+                         int64_t K, int out_dtype, void* out, void* stream) {
+  if (M < 0 || N <= 0 || K <= 0) return TG_ERR_INVALID_ARG;
+  if (!is_dtype(out_dtype) || !is_dtype(wscale_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
+  if (group != 32 && group != 64 && group != 128 && group != 256) return TG_ERR_UNSUPPORTED;
+  if (M > TG_INT4_MAX_M || K % 128 != 0 || K % group != 0) return TG_ERR_UNSUPPORTED;
+  if (N >= (int64_t(1) << 31) || K >= (int64_t(1) << 31)) return TG_ERR_UNSUPPORTED;
+  if (M == 0) return TG_OK;
+  if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
+  if (!aligned16(xq) || !aligned16(w4)) return TG_ERR_MISALIGNED;
+  if (!aligned_to(xscale, 4) || !aligned_to(wscale, dtype_bytes(wscale_dtype)) ||
+      !aligned_to(out, dtype_bytes(out_dtype)) || (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
+    return TG_ERR_MISALIGNED;
+  tg::GemvI4Params p;
+  p.xq = xq;
+  p.xscale = xscale;
+  p.w4 = w4;
+  p.wscale = wscale;
+  p.bias = bias;
+  p.wscale_dtype = wscale_dtype;
+  p.bias_dtype = bias_dtype;
+  p.group = group;
+  p.M = int(M);
+  p.N = int(N);
+  p.K = int(K);
+  p.out = out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid{unsigned((N + tg::gemv4::WARPS - 1) / tg::gemv4::WARPS)};
+  switch (out_dtype) {
+    case TG_DT_F32: return launch_dependent(tg::gemv_i4_kernel<0>, p, grid, tg::gemv4::THREADS, 0, st);
+    case TG_DT_F16: return launch_dependent(tg::gemv_i4_kernel<1>, p, grid, tg::gemv4::THREADS, 0, st);
+    default: return launch_dependent(tg::gemv_i4_kernel<2>, p, grid, tg::gemv4::THREADS, 0, st);
+  }
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------ routed experts
+namespace {
+
+// Tokens per CTA of the router: a warp's eight tokens at most where the
+// tokens are few, more where the CTAs' counts would become many.
+int route_per_block(int64_t T) {
+  int64_t per = 32;
+  while ((T + per - 1) / per > 256) per += 32;
+  return int(per);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tg_route_experts_workspace(int64_t T, int64_t E) {
+  if (T <= 0 || E <= 0) return 0;
+  const int per = route_per_block(T);
+  return size_t((T + per - 1) / per) * size_t(E) * 4;
+}
+
+int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int top_k, int renormalize,
+                     float* weights, int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* place, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (T < 0 || E <= 0 || top_k <= 0 || top_k > E || !is_dtype(dtype)) return TG_ERR_INVALID_ARG;
+  if (E > tg::route::MAX_E || top_k > tg::route::MAX_K) return TG_ERR_UNSUPPORTED;
+  if (T * top_k >= (int64_t(1) << 31)) return TG_ERR_UNSUPPORTED;
+  if (!offsets || !aligned_to(offsets, 4)) return offsets ? TG_ERR_MISALIGNED : TG_ERR_INVALID_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0)
+    return cudaMemsetAsync(offsets, 0, size_t(E + 1) * 4, st) == cudaSuccess ? TG_OK : TG_ERR_CUDA;
+  if (!logits || !weights || !ids || !rows || !place || !workspace) return TG_ERR_INVALID_ARG;
+  if (!aligned_to(logits, dtype_bytes(dtype)) || !aligned_to(weights, 4) || !aligned_to(ids, 4) ||
+      !aligned_to(rows, 4) || !aligned_to(place, 4) || !aligned_to(workspace, 4))
+    return TG_ERR_MISALIGNED;
+  if (workspace_bytes < tg_route_experts_workspace(T, E)) return TG_ERR_INVALID_ARG;
+  tg::RouteParams p;
+  p.logits = logits;
+  p.dtype = dtype;
+  p.T = int(T);
+  p.E = int(E);
+  p.top_k = top_k;
+  p.renormalize = renormalize != 0;
+  p.per_block = route_per_block(T);
+  p.blocks = int((T + p.per_block - 1) / p.per_block);
+  p.weights = weights;
+  p.ids = ids;
+  p.offsets = offsets;
+  p.rows = rows;
+  p.place = place;
+  p.counts = static_cast<int32_t*>(workspace);
+  const dim3 grid{unsigned(p.blocks)};
+  const int rc = launch_dependent(tg::route_topk_kernel, p, grid, tg::route::THREADS, 0, st);
+  if (rc != TG_OK) return rc;
+  return launch_dependent(tg::route_place_kernel, p, grid, tg::route::THREADS, 0, st);
+}
+
+int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place, const float* weights, int64_t T,
+                       int top_k, const void* residual, int64_t N, void* out, void* stream) {
+  if (T < 0 || R < 0 || N <= 0 || top_k <= 0 || !is_dtype(dtype)) return TG_ERR_INVALID_ARG;
+  if (top_k > tg::route::MAX_K || T >= (int64_t(1) << 31) || N >= (int64_t(1) << 31) || R >= (int64_t(1) << 31))
+    return TG_ERR_UNSUPPORTED;
+  if (T == 0) return TG_OK;
+  if ((!y && R > 0) || !place || !weights || !out) return TG_ERR_INVALID_ARG;
+  const size_t esz = dtype_bytes(dtype);
+  if (!aligned_to(y, esz) || !aligned_to(out, esz) || !aligned_to(residual, esz) || !aligned_to(place, 4) ||
+      !aligned_to(weights, 4))
+    return TG_ERR_MISALIGNED;
+  tg::CombineParams p;
+  p.y = y;
+  p.place = place;
+  p.weights = weights;
+  p.residual = residual;
+  p.out = out;
+  p.R = R;
+  p.T = T;
+  p.N = N;
+  p.top_k = top_k;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid{unsigned(T)};
+  switch (dtype) {
+    case TG_DT_F32: return launch_dependent(tg::combine_kernel<0>, p, grid, 256, 0, st);
+    case TG_DT_F16: return launch_dependent(tg::combine_kernel<1>, p, grid, 256, 0, st);
+    default: return launch_dependent(tg::combine_kernel<2>, p, grid, 256, 0, st);
+  }
+}
+
+int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t M, const int8_t* wq,
+                                 const float* wscale, int64_t wscale_numel, const void* bias, int bias_dtype,
+                                 const int32_t* rows, const int32_t* offsets, int64_t R, int64_t E, int64_t N,
+                                 int64_t K, int out_dtype, void* out, void* stream) {
+  if (M < 0 || R < 0 || E <= 0 || N <= 0 || K <= 0) return TG_ERR_INVALID_ARG;
+  if (!is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
+  if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
+  if (!rows && R > M) return TG_ERR_INVALID_ARG;
+  if (K % 16 != 0 || (N * int64_t(dtype_bytes(out_dtype))) % 16 != 0) return TG_ERR_UNSUPPORTED;
+  if (E > tg::route::MAX_E || M >= (int64_t(1) << 31) || R >= (int64_t(1) << 31) || K >= (int64_t(1) << 31) ||
+      N >= (int64_t(1) << 31) || E * N >= (int64_t(1) << 31))
+    return TG_ERR_UNSUPPORTED;
+  if (R == 0) return TG_OK;
+  if (!xscale || !wq || !wscale || !offsets || !out || (!xq && M > 0)) return TG_ERR_INVALID_ARG;
+  if (!aligned16(xq) || !aligned16(wq) || !aligned16(out)) return TG_ERR_MISALIGNED;
+  if (!aligned_to(xscale, 4) || !aligned_to(wscale, 4) || !aligned_to(rows, 4) || !aligned_to(offsets, 4) ||
+      (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
+    return TG_ERR_MISALIGNED;
+  using namespace tg::grouped;
+  tg::GroupedParams p;
+  p.xq = xq;
+  p.xscale = xscale;
+  p.wq = wq;
+  p.wscale = wscale;
+  p.bias = bias;
+  p.rows = rows;
+  p.offsets = offsets;
+  p.bias_dtype = bias_dtype;
+  p.wscale_mode = wscale_numel == 1 ? 0 : (wscale_numel == E * N ? 2 : 1);
+  p.M = M;
+  p.R = int(R);
+  p.E = int(E);
+  p.N = int(N);
+  p.K = int(K);
+  p.out = out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // No more tiles than full ones plus a part-filled one for each expert with rows.
+  const int64_t tiles = R / BM + std::min<int64_t>(E, R);
+  const int64_t cols = (N + BN - 1) / BN;
+  if (tiles > 65535) return TG_ERR_UNSUPPORTED;
+  const dim3 grid{unsigned(cols), unsigned(tiles)};
+  switch (out_dtype) {
+    case TG_DT_F32: return launch_dependent(tg::grouped_simple_kernel<0>, p, grid, THREADS, 0, st);
+    case TG_DT_F16: return launch_dependent(tg::grouped_simple_kernel<1>, p, grid, THREADS, 0, st);
+    default: return launch_dependent(tg::grouped_simple_kernel<2>, p, grid, THREADS, 0, st);
+  }
 }
 
 }  // extern "C"

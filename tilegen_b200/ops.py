@@ -18,6 +18,7 @@ as opaque ops).
 from __future__ import annotations
 
 import contextlib
+from typing import NamedTuple
 
 import torch
 
@@ -314,6 +315,239 @@ def _splitk_workspace(dev: torch.device, m: int, n: int) -> torch.Tensor:
     return ws
 
 
+# Most activation rows int4_gemv_dequant takes (TG_INT4_MAX_M); the groups of
+# input channels that share a scale; the router's limits.
+INT4_MAX_M = 64
+INT4_GROUPS = (32, 64, 128, 256)
+MAX_EXPERTS = 1024
+MAX_TOP_K = 32
+
+
+def _on(fn: str, name: str, t, dev: torch.device, dtypes, ndim: int) -> None:
+    """``t`` is a tensor on ``dev`` of one of ``dtypes`` and of ``ndim`` dimensions, or ValueError."""
+    if not isinstance(t, torch.Tensor) or t.device != dev:
+        raise ValueError(f"{fn}: {name} must be a tensor on {dev}")
+    if t.dtype not in dtypes or t.ndim != ndim:
+        raise ValueError(f"{fn}: {name} must be {ndim}-D of {' / '.join(map(str, dtypes))}, got {tuple(t.shape)} "
+                         f"{t.dtype}")
+
+
+def _no_grad(fn: str, *tensors) -> None:
+    """The forms for serving have no backward pass: an input that wants a gradient is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{fn}: no gradient is computed; call it under torch.no_grad() or on detached tensors")
+
+
+def _out(fn: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, dev: torch.device,
+         align: int = 16) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if (tuple(out.shape) != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous()
+            or out.data_ptr() % align):
+        raise ValueError(f"{fn}: out must be a contiguous {align}-byte aligned {list(shape)} {dtype} tensor on {dev}")
+    return out
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor,
+                      bias: torch.Tensor | None, out_dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Few rows of int8 codes times a 4-bit weight with group scales (``tg_int4_gemv_dequant``):
+    ``out[m, n] = (sum_g wscale[n, g] * (xq[m, g] . w4[n, g])) * xscale[m] + bias[n]``.
+
+    ``xq [M, K]`` int8 with ``xscale [M]`` as the quantisers return them, ``M`` at
+    most ``INT4_MAX_M``; ``w4 [N, K/2]`` uint8 in the layout of
+    ``tilegen_b200.quant.pack_int4`` and ``wscale [N, K/group]`` fp32/fp16/bf16 as
+    ``quantize_convrot_weight_int4`` returns them (``group``, read off the shapes,
+    32, 64, 128 or 256; ``K`` a multiple of 128); ``bias [N]`` or None.  A row's
+    result does not depend on the other rows.  ``out``: an optional contiguous
+    ``[M, N]`` ``out_dtype`` tensor to write into.
+    """
+    fn = "int4_gemv_dequant"
+    if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
+        raise ValueError(f"{fn}: CUDA tensors required")
+    dev = xq.device
+    _on(fn, "xq", xq, dev, (torch.int8,), 2)
+    _on(fn, "xscale", xscale, dev, (torch.float32,), 1)
+    _on(fn, "w4", w4, dev, (torch.uint8,), 2)
+    _on(fn, "wscale", wscale, dev, _FLOATS, 2)
+    if out_dtype not in _DTYPE_CODE:
+        raise ValueError(f"{fn}: unsupported out_dtype {out_dtype}")
+    m, k = xq.shape
+    n = w4.shape[0]
+    if m > INT4_MAX_M:
+        raise ValueError(f"{fn}: {m} rows, at most {INT4_MAX_M}")
+    if k % 128 or k == 0 or n == 0 or w4.shape[1] * 2 != k:
+        raise ValueError(f"{fn}: w4 {tuple(w4.shape)} does not match K={k} (a multiple of 128, two codes a byte)")
+    groups = wscale.shape[1]
+    if wscale.shape[0] != n or groups == 0 or k % groups or k // groups not in INT4_GROUPS:
+        raise ValueError(f"{fn}: wscale {tuple(wscale.shape)} is not [N, K / group] with group one of {INT4_GROUPS}")
+    if xscale.shape[0] != m:
+        raise ValueError(f"{fn}: xscale has {xscale.shape[0]} elements, expected {m}")
+    b_ptr, b_code = None, _lib.TG_DT_F32
+    if bias is not None:
+        _on(fn, "bias", bias, dev, _FLOATS, 1)
+        if bias.shape[0] != n:
+            raise ValueError(f"{fn}: bias has {bias.shape[0]} elements, expected {n}")
+        bias = bias.contiguous()
+        b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
+    _no_grad(fn, xscale, wscale, bias)
+    xq, w4, xscale, wscale = _aligned(xq), _aligned(w4), xscale.contiguous(), wscale.contiguous()
+    out = _out(fn, out, (m, n), out_dtype, dev)
+    if m:
+        _call("tg_int4_gemv_dequant", dev, xq.data_ptr(), xscale.data_ptr(), w4.data_ptr(), wscale.data_ptr(),
+              _DTYPE_CODE[wscale.dtype], k // groups, b_ptr, b_code, m, n, k, _DTYPE_CODE[out_dtype], out.data_ptr())
+    return out
+
+
+class ExpertRoutes(NamedTuple):
+    """What ``route_experts`` returns; ``T`` tokens, ``k`` experts each."""
+
+    weights: torch.Tensor  # [T, k] fp32
+    ids: torch.Tensor      # [T, k] int32, -1 where a slot is left out
+    offsets: torch.Tensor  # [E + 1] int32: expert e's rows are offsets[e] .. offsets[e + 1] - 1
+    rows: torch.Tensor     # [T * k] int32: row r's token, -1 behind the last row
+    place: torch.Tensor    # [T, k] int32: the row of each slot, -1 where it is left out
+
+
+def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> ExpertRoutes:
+    """The router of a layer with routed experts (``tg_route_experts``): of ``logits
+    [T, E]`` (fp32/fp16/bf16) each token's ``top_k`` experts -- largest first, equal
+    logits by ascending index, NaN above everything -- with their softmax weights
+    over the chosen experts (``renormalize``) or over all, and the (token, expert)
+    slots sorted by expert, then token.  A slot whose logit is -inf (a closed expert,
+    a padded token) is left out.  Nothing is read back to the host: ``offsets`` and
+    ``rows`` go to ``int8_grouped_gemm_dequant`` and ``place`` and ``weights`` to
+    ``combine_experts`` as they are.
+    """
+    fn = "route_experts"
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError(f"{fn}: CUDA tensor required")
+    dev = logits.device
+    _on(fn, "logits", logits, dev, _FLOATS, 2)
+    t, e = logits.shape
+    top_k = int(top_k)
+    if not 1 <= e <= MAX_EXPERTS:
+        raise ValueError(f"{fn}: {e} experts, 1 to {MAX_EXPERTS} are supported")
+    if not 1 <= top_k <= min(e, MAX_TOP_K):
+        raise ValueError(f"{fn}: top_k={top_k} must be 1 to {min(e, MAX_TOP_K)}")
+    if t * top_k >= 1 << 31:
+        raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
+    _no_grad(fn, logits)
+    logits = logits.contiguous()
+    weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    offsets = torch.empty((e + 1,), dtype=torch.int32, device=dev)
+    rows = torch.empty((t * top_k,), dtype=torch.int32, device=dev)
+    place = torch.empty((t, top_k), dtype=torch.int32, device=dev)
+    need = int(_lib.lib().tg_route_experts_workspace(t, e))
+    work = torch.empty((need,), dtype=torch.uint8, device=dev)
+    _call("tg_route_experts", dev, logits.data_ptr(), _DTYPE_CODE[logits.dtype], t, e, top_k, int(bool(renormalize)),
+          weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), place.data_ptr(), work.data_ptr(),
+          need)
+    return ExpertRoutes(weights, ids, offsets, rows, place)
+
+
+def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor,
+                              bias: torch.Tensor | None, offsets: torch.Tensor, out_dtype: torch.dtype,
+                              rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``int8_gemm_dequant`` with one weight per expert over ragged groups of rows
+    (``tg_int8_grouped_gemm_dequant``): for ``offsets[e] <= r < offsets[e + 1]`` and
+    ``a = rows[r]`` (``r`` without ``rows``),
+    ``out[r] = ((float(xq[a] @ wq[e].T) * xscale[a]) * wscale[e]) + bias[e]``.
+
+    ``xq [M, K]`` int8, ``xscale [M]``; ``wq [E, N, K]`` int8; ``wscale`` one scale,
+    ``[E]`` or ``[E, N]`` fp32; ``bias [E, N]`` or None; ``offsets [E + 1]`` and ``rows
+    [R]`` int32, as ``route_experts`` returns them.  ``out``: an optional contiguous
+    ``[R, N]`` ``out_dtype`` tensor to write into; rows that no group covers are left
+    as they were (uninitialised when ``out`` is not given).  Each row is
+    bit-identical to ``int8_gemm_dequant`` with its expert's weight.
+    """
+    fn = "int8_grouped_gemm_dequant"
+    if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
+        raise ValueError(f"{fn}: CUDA tensors required")
+    dev = xq.device
+    _on(fn, "xq", xq, dev, (torch.int8,), 2)
+    _on(fn, "xscale", xscale, dev, (torch.float32,), 1)
+    _on(fn, "wq", wq, dev, (torch.int8,), 3)
+    _on(fn, "offsets", offsets, dev, (torch.int32,), 1)
+    if out_dtype not in _DTYPE_CODE:
+        raise ValueError(f"{fn}: unsupported out_dtype {out_dtype}")
+    m, k = xq.shape
+    e, n, kw = wq.shape
+    if not 1 <= e <= MAX_EXPERTS:
+        raise ValueError(f"{fn}: {e} experts, 1 to {MAX_EXPERTS} are supported")
+    if kw != k or k == 0 or n == 0:
+        raise ValueError(f"{fn}: shapes {tuple(xq.shape)} x {tuple(wq.shape)}^T do not match")
+    if offsets.shape[0] != e + 1:
+        raise ValueError(f"{fn}: offsets has {offsets.shape[0]} elements, expected {e + 1}")
+    if xscale.shape[0] != m:
+        raise ValueError(f"{fn}: xscale has {xscale.shape[0]} elements, expected {m}")
+    if not isinstance(wscale, torch.Tensor) or wscale.device != dev or wscale.dtype != torch.float32 \
+            or wscale.numel() not in (1, e, e * n):
+        raise ValueError(f"{fn}: wscale must be fp32 on {dev} with 1, {e} or {e} x {n} elements")
+    b_ptr, b_code = None, _lib.TG_DT_F32
+    if bias is not None:
+        _on(fn, "bias", bias, dev, _FLOATS, 2)
+        if tuple(bias.shape) != (e, n):
+            raise ValueError(f"{fn}: bias is {tuple(bias.shape)}, expected {(e, n)}")
+        bias = bias.contiguous()
+        b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
+    r, r_ptr = m, None
+    if rows is not None:
+        _on(fn, "rows", rows, dev, (torch.int32,), 1)
+        rows = rows.contiguous()
+        r, r_ptr = rows.shape[0], rows.data_ptr()
+    _no_grad(fn, xscale, wscale, bias)
+    xq, wq = _aligned(xq), _aligned(wq)
+    xscale, wscale, offsets = xscale.contiguous(), wscale.contiguous(), offsets.contiguous()
+    out = _out(fn, out, (r, n), out_dtype, dev)
+    if r:
+        _call("tg_int8_grouped_gemm_dequant", dev, xq.data_ptr(), xscale.data_ptr(), m, wq.data_ptr(),
+              wscale.data_ptr(), wscale.numel(), b_ptr, b_code, r_ptr, offsets.data_ptr(), r, e, n, k,
+              _DTYPE_CODE[out_dtype], out.data_ptr())
+    return out
+
+
+def combine_experts(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor,
+                    residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Each token's experts' rows added up (``tg_combine_experts``): ``out[t] = sum_j
+    weights[t, j] * y[place[t, j]] (+ residual[t])`` in fp32, rounded once to ``y``'s dtype.
+
+    ``y [R, N]`` fp32/fp16/bf16; ``place [T, k]`` int32 and ``weights [T, k]`` fp32 as
+    ``route_experts`` returns them (a place outside ``[0, R)`` adds nothing);
+    ``residual [T, N]`` of ``y``'s dtype or None.  ``out``: an optional contiguous ``[T,
+    N]`` tensor to write into, which may be ``residual`` itself.
+    """
+    fn = "combine_experts"
+    if not isinstance(y, torch.Tensor) or not y.is_cuda:
+        raise ValueError(f"{fn}: CUDA tensors required")
+    dev = y.device
+    _on(fn, "y", y, dev, _FLOATS, 2)
+    _on(fn, "place", place, dev, (torch.int32,), 2)
+    _on(fn, "weights", weights, dev, (torch.float32,), 2)
+    r, n = y.shape
+    t, top_k = place.shape
+    if weights.shape != place.shape or not 1 <= top_k <= MAX_TOP_K:
+        raise ValueError(f"{fn}: place {tuple(place.shape)} and weights {tuple(weights.shape)} must be [T, k] with k "
+                         f"1 to {MAX_TOP_K}")
+    if n == 0:
+        raise ValueError(f"{fn}: y has no columns")
+    if residual is not None:
+        _on(fn, "residual", residual, dev, (y.dtype,), 2)
+        if tuple(residual.shape) != (t, n):
+            raise ValueError(f"{fn}: residual is {tuple(residual.shape)}, expected {(t, n)}")
+        residual = residual.contiguous()
+    _no_grad(fn, y, weights, residual)
+    y, place, weights = y.contiguous(), place.contiguous(), weights.contiguous()
+    out = _out(fn, out, (t, n), y.dtype, dev, y.element_size())
+    if t:
+        _call("tg_combine_experts", dev, y.data_ptr(), _DTYPE_CODE[y.dtype], r, place.data_ptr(), weights.data_ptr(),
+              t, top_k, None if residual is None else residual.data_ptr(), n, out.data_ptr())
+    return out
+
+
 # ---------------------------------------------------------------- custom ops
 @torch.library.custom_op("tilegen::rotate_quant", mutates_args=())
 def _rotate_quant_op(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -356,3 +590,51 @@ def _int8_gemm_dequant_op(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.Tens
 @_int8_gemm_dequant_op.register_fake
 def _(xq, xscale, wq, wscale, bias, out_dtype):
     return xq.new_empty((xq.shape[0], wq.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("tilegen::int4_gemv_dequant", mutates_args=())
+def _int4_gemv_dequant_op(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor,
+                          bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
+    return int4_gemv_dequant(xq, xscale, w4, wscale, bias, out_dtype)
+
+
+@_int4_gemv_dequant_op.register_fake
+def _(xq, xscale, w4, wscale, bias, out_dtype):
+    return xq.new_empty((xq.shape[0], w4.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("tilegen::route_experts", mutates_args=())
+def _route_experts_op(logits: torch.Tensor, top_k: int, renormalize: bool) -> tuple[
+        torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(route_experts(logits, top_k, renormalize))
+
+
+@_route_experts_op.register_fake
+def _(logits, top_k, renormalize):
+    t, e = logits.shape
+    return (logits.new_empty((t, top_k), dtype=torch.float32), logits.new_empty((t, top_k), dtype=torch.int32),
+            logits.new_empty((e + 1,), dtype=torch.int32), logits.new_empty((t * top_k,), dtype=torch.int32),
+            logits.new_empty((t, top_k), dtype=torch.int32))
+
+
+@torch.library.custom_op("tilegen::int8_grouped_gemm_dequant", mutates_args=())
+def _int8_grouped_gemm_dequant_op(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor,
+                                  bias: torch.Tensor | None, offsets: torch.Tensor, out_dtype: torch.dtype,
+                                  rows: torch.Tensor | None) -> torch.Tensor:
+    return int8_grouped_gemm_dequant(xq, xscale, wq, wscale, bias, offsets, out_dtype, rows)
+
+
+@_int8_grouped_gemm_dequant_op.register_fake
+def _(xq, xscale, wq, wscale, bias, offsets, out_dtype, rows):
+    return xq.new_empty(((xq if rows is None else rows).shape[0], wq.shape[1]), dtype=out_dtype)
+
+
+@torch.library.custom_op("tilegen::combine_experts", mutates_args=())
+def _combine_experts_op(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor,
+                        residual: torch.Tensor | None) -> torch.Tensor:
+    return combine_experts(y, place, weights, residual)
+
+
+@_combine_experts_op.register_fake
+def _(y, place, weights, residual):
+    return y.new_empty((place.shape[0], y.shape[1]))
