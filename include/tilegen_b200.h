@@ -223,14 +223,15 @@ int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
  *
  *   out[m,n] = (sum_g wscale[n,g] * float(sum_{k in g} xq[m,k] * w4[n,k])) * xscale[m] + bias[n]
  *
- * The inner sums are exact, the outer one is fp32, in an order that depends on
- * N and K only (a row's result does not depend on the other rows or on M).
+ * The inner sums are exact (a group of 256: each half's), the outer one is fp32
+ * in an order that depends on K only (a row's result does not depend on the
+ * other rows or on M).
  *
  *   xq      [M, K] int8, 16-B aligned; K % 128 == 0
  *   w4      [N, K/2] bytes, 16-B aligned: of each 128 codes of a row, byte
  *           16 t + 4 j + b (t, j, b = 0..3) holds code 32 j + 8 t + b in its low
  *           and code 32 j + 8 t + 4 + b in its high half, two's complement
- *   wscale  [N, K/group] of wscale_dtype (TG_DT_F32/F16/BF16)
+ *   wscale  [N, K/group] of wscale_dtype (TG_DT_F32/F16/BF16), 16-B aligned
  *   group   32, 64, 128 or 256 consecutive codes; K % group == 0
  *   bias    [N] of bias_dtype or NULL; out [M, N] of out_dtype (any N)
  * M == 0 is a no-op; TG_ERR_UNSUPPORTED for M > TG_INT4_MAX_M.

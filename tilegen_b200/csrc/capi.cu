@@ -1094,6 +1094,25 @@ int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, 
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
+template <int MT, int RT, int SV, bool S4>
+int launch_gemv4_t(const tg::GemvI4Params& p, int dev, cudaStream_t st) {
+  static uint32_t attr_done[kMaxDevices];
+  auto kern = tg::gemv_i4_kernel<MT, RT, SV, S4>;
+  constexpr uint32_t smem = tg::gemv4::smem_bytes(MT, RT);
+  if (!ensure_smem_attr(kern, dev, smem, attr_done)) return TG_ERR_CUDA;
+  return launch_dependent(kern, p, dim3(unsigned((int64_t(p.N) + RT * 16 - 1) / (RT * 16))), tg::gemv4::THREADS, smem, st);
+}
+
+// sv: scales per block of 128 codes.
+template <int MT, int RT>
+int launch_gemv4_s(const tg::GemvI4Params& p, int sv, bool s4, int dev, cudaStream_t st) {
+  switch (sv) {
+    case 4: return s4 ? launch_gemv4_t<MT, RT, 4, true>(p, dev, st) : launch_gemv4_t<MT, RT, 4, false>(p, dev, st);
+    case 2: return s4 ? launch_gemv4_t<MT, RT, 2, true>(p, dev, st) : launch_gemv4_t<MT, RT, 2, false>(p, dev, st);
+    default: return s4 ? launch_gemv4_t<MT, RT, 1, true>(p, dev, st) : launch_gemv4_t<MT, RT, 1, false>(p, dev, st);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -1108,9 +1127,8 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (N >= (int64_t(1) << 31) || K >= (int64_t(1) << 31)) return TG_ERR_UNSUPPORTED;
   if (M == 0) return TG_OK;
   if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
-  if (!aligned16(xq) || !aligned16(w4)) return TG_ERR_MISALIGNED;
-  if (!aligned_to(xscale, 4) || !aligned_to(wscale, dtype_bytes(wscale_dtype)) ||
-      !aligned_to(out, dtype_bytes(out_dtype)) || (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
+  if (!aligned16(xq) || !aligned16(w4) || !aligned16(wscale)) return TG_ERR_MISALIGNED;
+  if (!aligned_to(xscale, 4) || !aligned_to(out, dtype_bytes(out_dtype)) || (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
     return TG_ERR_MISALIGNED;
   tg::GemvI4Params p;
   p.xq = xq;
@@ -1120,18 +1138,25 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   p.bias = bias;
   p.wscale_dtype = wscale_dtype;
   p.bias_dtype = bias_dtype;
-  p.group = group;
+  p.out_dtype = out_dtype;
+  p.groups = int(K / group);
+  p.scale_shift = group == 256 ? 1 : 0;
   p.M = int(M);
   p.N = int(N);
   p.K = int(K);
+  // A quarter of each row, as the int8 GEMV.
+  p.prefetch = N * K / 2 <= kGemvPrefetchMaxBytes ? int(K / 8 / 16 * 16) : 0;
   p.out = out;
+  int dev;
+  DeviceInfo info;
+  if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid{unsigned((N + tg::gemv4::WARPS - 1) / tg::gemv4::WARPS)};
-  switch (out_dtype) {
-    case TG_DT_F32: return launch_dependent(tg::gemv_i4_kernel<0>, p, grid, tg::gemv4::THREADS, 0, st);
-    case TG_DT_F16: return launch_dependent(tg::gemv_i4_kernel<1>, p, grid, tg::gemv4::THREADS, 0, st);
-    default: return launch_dependent(tg::gemv_i4_kernel<2>, p, grid, tg::gemv4::THREADS, 0, st);
-  }
+  const int sv = group == 32 ? 4 : (group == 64 ? 2 : 1);
+  const bool s4 = wscale_dtype == TG_DT_F32;
+  if (M <= 8) return launch_gemv4_s<1, 1>(p, sv, s4, dev, st);
+  if (M <= 16) return launch_gemv4_s<2, 2>(p, sv, s4, dev, st);
+  if (M <= 32) return launch_gemv4_s<4, 2>(p, sv, s4, dev, st);
+  return launch_gemv4_s<8, 2>(p, sv, s4, dev, st);
 }
 
 }  // extern "C"

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
       acc = fmaf(p.weights[t * p.top_k + j], load_as_f32(p.y, DT, size_t(r) * p.N + n), acc);
     }
     if (p.residual) acc += load_as_f32(p.residual, DT, size_t(t) * p.N + n);
-    store_f32_as<DT>(p.out, size_t(t) * p.N + n, acc);
+    store_f32_as(p.out, DT, size_t(t) * p.N + n, acc);
   }
 }
 

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(grouped::THREADS) grouped_simple_kernel(const 
       const float ws = p.wscale[p.wscale_mode == 0 ? 0 : (p.wscale_mode == 1 ? size_t(e) : en)];
       float v = __fmul_rn(__fmul_rn(__int2float_rn(acc[a][b]), xs), ws);
       if (p.bias) v = __fadd_rn(v, load_as_f32(p.bias, p.bias_dtype, en));
-      store_f32_as<OUT>(p.out, size_t(r) * p.N + n, v);
+      store_f32_as(p.out, OUT, size_t(r) * p.N + n, v);
     }
   }
 }

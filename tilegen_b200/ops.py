@@ -393,7 +393,7 @@ def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, 
         bias = bias.contiguous()
         b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
     _no_grad(fn, xscale, wscale, bias)
-    xq, w4, xscale, wscale = _aligned(xq), _aligned(w4), xscale.contiguous(), wscale.contiguous()
+    xq, w4, xscale, wscale = _aligned(xq), _aligned(w4), xscale.contiguous(), _aligned(wscale)
     out = _out(fn, out, (m, n), out_dtype, dev)
     if m:
         _call("tg_int4_gemv_dequant", dev, xq.data_ptr(), xscale.data_ptr(), w4.data_ptr(), wscale.data_ptr(),
