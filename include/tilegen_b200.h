@@ -275,7 +275,7 @@ size_t tg_route_experts_workspace(int64_t T, int64_t E);
  *   out[r,n] = ((float(sum_k xq[a,k] * wq[e,n,k]) * xscale[a]) * wscale[e,n]) + bias[e,n]
  * each row bit-identical to tg_int8_gemm_dequant with that expert's weight.
  *
- *   xq       [M, K] int8, xscale [M]; K % 16 == 0
+ *   xq       [M, K] int8, xscale [M]; K % 16 == 0; M >= 1 unless R == 0
  *   wq       [E, N, K] int8; wscale fp32 of 1, E or E*N elements
  *   bias     [E, N] of bias_dtype or NULL
  *   rows     [R] row of xq behind each output row, or NULL (then R <= M); an

@@ -1248,6 +1248,51 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
   }
 }
 
+}  // extern "C"
+
+namespace {
+
+template <int TN, int OUT, bool GATHER>
+int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const tg::GroupedParams& p, int dev, int sms,
+                     cudaStream_t st) {
+  static uint32_t attr_done[kMaxDevices];
+  constexpr uint32_t smem = tg::grouped::smem_bytes(TN);
+  auto kern = tg::gemm_i8_grouped_kernel<TN, OUT, GATHER>;
+  if (!ensure_smem_attr(kern, dev, smem, attr_done)) return TG_ERR_CUDA;
+  // No more tiles than the full ones and a part-filled one for each expert.
+  const int64_t most = (int64_t(p.R) / TN + std::min<int64_t>(p.E, p.R)) * p.n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(sms, most)));
+  cfg.blockDim = dim3(tg::grouped::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, tw, tx, p) != cudaSuccess) return TG_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
+}
+
+template <int TN>
+int launch_grouped_tn(const CUtensorMap& tw, const CUtensorMap& tx, const tg::GroupedParams& p, int out_dtype, int dev,
+                      int sms, cudaStream_t st) {
+  const bool g = p.rows != nullptr;
+  switch (out_dtype) {
+    case TG_DT_F32: return g ? launch_grouped_t<TN, 0, true>(tw, tx, p, dev, sms, st)
+                             : launch_grouped_t<TN, 0, false>(tw, tx, p, dev, sms, st);
+    case TG_DT_F16: return g ? launch_grouped_t<TN, 1, true>(tw, tx, p, dev, sms, st)
+                             : launch_grouped_t<TN, 1, false>(tw, tx, p, dev, sms, st);
+    default: return g ? launch_grouped_t<TN, 2, true>(tw, tx, p, dev, sms, st)
+                      : launch_grouped_t<TN, 2, false>(tw, tx, p, dev, sms, st);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
 int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t M, const int8_t* wq,
                                  const float* wscale, int64_t wscale_numel, const void* bias, int bias_dtype,
                                  const int32_t* rows, const int32_t* offsets, int64_t R, int64_t E, int64_t N,
@@ -1255,45 +1300,50 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   if (M < 0 || R < 0 || E <= 0 || N <= 0 || K <= 0) return TG_ERR_INVALID_ARG;
   if (!is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
   if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
-  if (!rows && R > M) return TG_ERR_INVALID_ARG;
+  if ((!rows && R > M) || (R > 0 && M == 0)) return TG_ERR_INVALID_ARG;
   if (K % 16 != 0 || (N * int64_t(dtype_bytes(out_dtype))) % 16 != 0) return TG_ERR_UNSUPPORTED;
   if (E > tg::route::MAX_E || M >= (int64_t(1) << 31) || R >= (int64_t(1) << 31) || K >= (int64_t(1) << 31) ||
       N >= (int64_t(1) << 31) || E * N >= (int64_t(1) << 31))
     return TG_ERR_UNSUPPORTED;
   if (R == 0) return TG_OK;
-  if (!xscale || !wq || !wscale || !offsets || !out || (!xq && M > 0)) return TG_ERR_INVALID_ARG;
+  if (!xq || !xscale || !wq || !wscale || !offsets || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(wq) || !aligned16(out)) return TG_ERR_MISALIGNED;
   if (!aligned_to(xscale, 4) || !aligned_to(wscale, 4) || !aligned_to(rows, 4) || !aligned_to(offsets, 4) ||
       (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
     return TG_ERR_MISALIGNED;
+  int dev;
+  DeviceInfo info;
+  if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   using namespace tg::grouped;
+  CUtensorMap tw, tx;
+  if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, uint64_t(K), uint64_t(E * N), uint64_t(K), BK, BNW,
+                    CU_TENSOR_MAP_SWIZZLE_128B))
+    return TG_ERR_CUDA;
+  if (!make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(K), uint64_t(M), uint64_t(K), BK,
+                    rows ? 1u : uint32_t(XBOX), CU_TENSOR_MAP_SWIZZLE_128B))
+    return TG_ERR_CUDA;
   tg::GroupedParams p;
-  p.xq = xq;
   p.xscale = xscale;
-  p.wq = wq;
   p.wscale = wscale;
   p.bias = bias;
   p.rows = rows;
   p.offsets = offsets;
   p.bias_dtype = bias_dtype;
   p.wscale_mode = wscale_numel == 1 ? 0 : (wscale_numel == E * N ? 2 : 1);
-  p.M = M;
+  p.M = int(M);
   p.R = int(R);
   p.E = int(E);
   p.N = int(N);
   p.K = int(K);
+  p.n_tiles = int((N + BNW - 1) / BNW);
+  p.k_blocks = int((K + BK - 1) / BK);
   p.out = out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // No more tiles than full ones plus a part-filled one for each expert with rows.
-  const int64_t tiles = R / BM + std::min<int64_t>(E, R);
-  const int64_t cols = (N + BN - 1) / BN;
-  if (tiles > 65535) return TG_ERR_UNSUPPORTED;
-  const dim3 grid{unsigned(cols), unsigned(tiles)};
-  switch (out_dtype) {
-    case TG_DT_F32: return launch_dependent(tg::grouped_simple_kernel<0>, p, grid, THREADS, 0, st);
-    case TG_DT_F16: return launch_dependent(tg::grouped_simple_kernel<1>, p, grid, THREADS, 0, st);
-    default: return launch_dependent(tg::grouped_simple_kernel<2>, p, grid, THREADS, 0, st);
-  }
+  // Rows an expert has on average, if every expert has some.
+  const int64_t avg = R / std::min<int64_t>(E, R);
+  if (avg <= 24) return launch_grouped_tn<32>(tw, tx, p, out_dtype, dev, info.sms, st);
+  if (avg <= 128) return launch_grouped_tn<128>(tw, tx, p, out_dtype, dev, info.sms, st);
+  return launch_grouped_tn<256>(tw, tx, p, out_dtype, dev, info.sms, st);
 }
 
 }  // extern "C"
