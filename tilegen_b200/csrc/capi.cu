@@ -1252,40 +1252,56 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
 
 namespace {
 
-template <int TN, int OUT, bool GATHER>
-int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const tg::GroupedParams& p, int dev, int sms,
-                     cudaStream_t st) {
+// The output's tensor map has to match the kernel's chunk (32 rows x 32 channels).
+template <int TN, int OUT, bool GATHER, bool PAIR>
+int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, tg::GroupedParams p, int dev,
+                     int sms, cudaStream_t st) {
   static uint32_t attr_done[kMaxDevices];
-  constexpr uint32_t smem = tg::grouped::smem_bytes(TN);
-  auto kern = tg::gemm_i8_grouped_kernel<TN, OUT, GATHER>;
+  using namespace tg::grouped;
+  constexpr uint32_t smem = smem_bytes(TN, PAIR);
+  auto kern = tg::gemm_i8_grouped_kernel<TN, OUT, GATHER, PAIR>;
   if (!ensure_smem_attr(kern, dev, smem, attr_done)) return TG_ERR_CUDA;
+  constexpr int kTileN = PAIR ? 2 * BNW : BNW;
+  constexpr int64_t kKBlock = int64_t(BK) * ksub(PAIR);
+  p.n_tiles = int((int64_t(p.N) + kTileN - 1) / kTileN);
+  p.k_blocks = int((int64_t(p.K) + kKBlock - 1) / kKBlock);
   // No more tiles than the full ones and a part-filled one for each expert.
   const int64_t most = (int64_t(p.R) / TN + std::min<int64_t>(p.E, p.R)) * p.n_tiles;
+  // The pair GEMM's clusters of two take as much shared memory: as many fit.
+  const int units = int(std::min<int64_t>(gemm_units(dev, sms, PAIR), most));
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(sms, most)));
-  cfg.blockDim = dim3(tg::grouped::THREADS);
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(unsigned(PAIR ? 2 * units : units));
+  cfg.blockDim = dim3(threads(GATHER));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, tw, tx, p) != cudaSuccess) return TG_ERR_CUDA;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, kern, tw, tx, to, p) != cudaSuccess) return TG_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-template <int TN>
-int launch_grouped_tn(const CUtensorMap& tw, const CUtensorMap& tx, const tg::GroupedParams& p, int out_dtype, int dev,
-                      int sms, cudaStream_t st) {
+template <int TN, bool PAIR>
+int launch_grouped_tn(const int8_t* xq, const CUtensorMap& tw, const CUtensorMap& to, const tg::GroupedParams& p,
+                      int out_dtype, int dev, int sms, cudaStream_t st) {
   const bool g = p.rows != nullptr;
+  CUtensorMap tx;
+  if (!make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(p.K), uint64_t(p.M), uint64_t(p.K),
+                    tg::grouped::BK, g ? 1u : uint32_t(tg::grouped::xbox(TN)), CU_TENSOR_MAP_SWIZZLE_128B))
+    return TG_ERR_CUDA;
   switch (out_dtype) {
-    case TG_DT_F32: return g ? launch_grouped_t<TN, 0, true>(tw, tx, p, dev, sms, st)
-                             : launch_grouped_t<TN, 0, false>(tw, tx, p, dev, sms, st);
-    case TG_DT_F16: return g ? launch_grouped_t<TN, 1, true>(tw, tx, p, dev, sms, st)
-                             : launch_grouped_t<TN, 1, false>(tw, tx, p, dev, sms, st);
-    default: return g ? launch_grouped_t<TN, 2, true>(tw, tx, p, dev, sms, st)
-                      : launch_grouped_t<TN, 2, false>(tw, tx, p, dev, sms, st);
+    case TG_DT_F32: return g ? launch_grouped_t<TN, 0, true, PAIR>(tw, tx, to, p, dev, sms, st)
+                             : launch_grouped_t<TN, 0, false, PAIR>(tw, tx, to, p, dev, sms, st);
+    case TG_DT_F16: return g ? launch_grouped_t<TN, 1, true, PAIR>(tw, tx, to, p, dev, sms, st)
+                             : launch_grouped_t<TN, 1, false, PAIR>(tw, tx, to, p, dev, sms, st);
+    default: return g ? launch_grouped_t<TN, 2, true, PAIR>(tw, tx, to, p, dev, sms, st)
+                      : launch_grouped_t<TN, 2, false, PAIR>(tw, tx, to, p, dev, sms, st);
   }
 }
 
@@ -1315,12 +1331,15 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   DeviceInfo info;
   if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   using namespace tg::grouped;
-  CUtensorMap tw, tx;
+  CUtensorMap tw, to;
   if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, uint64_t(K), uint64_t(E * N), uint64_t(K), BK, BNW,
                     CU_TENSOR_MAP_SWIZZLE_128B))
     return TG_ERR_CUDA;
-  if (!make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(K), uint64_t(M), uint64_t(K), BK,
-                    rows ? 1u : uint32_t(XBOX), CU_TENSOR_MAP_SWIZZLE_128B))
+  const CUtensorMapDataType odt = out_dtype == TG_DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : out_dtype == TG_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (!make_tmap_2d(&to, odt, out, uint64_t(N), uint64_t(R), uint64_t(N) * dtype_bytes(out_dtype), 32, 32,
+                    CU_TENSOR_MAP_SWIZZLE_NONE))
     return TG_ERR_CUDA;
   tg::GroupedParams p;
   p.xscale = xscale;
@@ -1335,15 +1354,13 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   p.E = int(E);
   p.N = int(N);
   p.K = int(K);
-  p.n_tiles = int((N + BNW - 1) / BNW);
-  p.k_blocks = int((K + BK - 1) / BK);
   p.out = out;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Rows an expert has on average, if every expert has some.
   const int64_t avg = R / std::min<int64_t>(E, R);
-  if (avg <= 24) return launch_grouped_tn<32>(tw, tx, p, out_dtype, dev, info.sms, st);
-  if (avg <= 128) return launch_grouped_tn<128>(tw, tx, p, out_dtype, dev, info.sms, st);
-  return launch_grouped_tn<256>(tw, tx, p, out_dtype, dev, info.sms, st);
+  if (avg <= 24) return launch_grouped_tn<32, false>(xq, tw, to, p, out_dtype, dev, info.sms, st);
+  if (avg <= 128) return launch_grouped_tn<128, false>(xq, tw, to, p, out_dtype, dev, info.sms, st);
+  return launch_grouped_tn<256, true>(xq, tw, to, p, out_dtype, dev, info.sms, st);
 }
 
 }  // extern "C"

@@ -7,22 +7,27 @@
 // each row is gemm_i8.cuh's, so a group's rows are bit-identical to
 // tg_int8_gemm_dequant on that expert's weight.
 //
-// Structure (persistent, one CTA per SM, 192 threads; roles as in gemm_i8.cuh):
+// Structure (persistent, one CTA per SM; roles as in gemm_i8.cuh: warp 0 TMA
+// producer, warp 1 MMA issuer, warps 2-5 epilogue; with gathered rows warps 6-8
+// are producers too):
 //  * The operands swap roles, as in gemm_splitk.cuh: a 128-row tile of an
 //    expert's WEIGHT is the UMMA M operand and up to TN of its activation rows
-//    are UMMA N.  N is set per tile (a multiple of 16), so a group of three
-//    rows costs a 16-column product and three rows' loads, not a 128-row
-//    tile's, and nothing of a neighbouring group is ever computed.
+//    are UMMA N.  N is set per tile (a multiple of 16, of 32 for pairs), so a
+//    group of three rows costs a 16-column product and three rows' loads, not
+//    a 128-row tile's, and nothing of a neighbouring group is ever computed.
+//  * PAIR: two CTAs of a cluster take 256 weight rows by the pair MMA; each
+//    loads its 128 weight rows and half of the activation rows.
 //  * The offsets stay on the device: each CTA turns them into a prefix sum of
-//    tiles per expert in shared memory, and its roles walk the tiles
-//    blockIdx.x, blockIdx.x + gridDim.x, ... by it.  An expert's rows are cut
-//    into equal token tiles, which run fastest, so tiles in flight share
-//    their weight rows in L2; an expert without rows has no tile.
-//  * Activation rows come by TMA, 16 rows a box, or with `rows` by
-//    tile::gather4 (box one row high): each lane of the producer warp
-//    holds the row numbers of its gathers and issues them.
-//  * The epilogue holds one output channel per lane and stores column by
-//    column (32 neighbouring channels of a row per warp and store).
+//    tiles per expert in shared memory, and its roles walk the tiles unit,
+//    unit + units, ... by it.  An expert's rows are cut into equal token tiles,
+//    which run fastest, so tiles in flight share their weight rows in L2; an
+//    expert without rows has no tile.
+//  * Activation rows come by TMA, XBOX rows a box, or with `rows` by
+//    tile::gather4 (box one row high).  One lane issuing a gather takes about 50
+//    cycles, so four warps share them.
+//  * The epilogue holds one output channel per lane and a row per column: it
+//    stages 32 rows x 32 channels a warp in shared memory for one TMA store, and
+//    stores the part-filled last chunk of a group directly, row by row.
 // What bounds it: few rows per expert, the used experts' weight bytes (HBM);
 // hundreds of rows, the int8 tensor rate.
 #pragma once
@@ -34,19 +39,28 @@
 namespace tg {
 
 namespace grouped {
-constexpr int THREADS = 192;
-constexpr int BNW = 128;                 // weight rows per tile (UMMA M)
+constexpr int BNW = 128;                 // weight rows per CTA (UMMA M per CTA)
 constexpr int BK = 128;                  // bytes of K per k-block
 constexpr int UK = 32;                   // K per tcgen05.mma kind::i8
 constexpr uint32_t W_BYTES = BNW * BK;   // 16 KB
-constexpr int XBOX = 16;                 // activation rows per TMA box
+constexpr int HELPERS = 3;               // producer warps beside warp 0 (gathered rows)
+constexpr int STAGE_OUT = 4096;          // epilogue staging bytes per warp
 constexpr int MAX_E = TG_MAX_EXPERTS;
-__host__ __device__ constexpr uint32_t stage_bytes(int tn) { return W_BYTES + uint32_t(tn) * BK; }
-__host__ __device__ constexpr int stages(int tn) {
-  return int(208u * 1024u / stage_bytes(tn)) > 10 ? 10 : int(208u * 1024u / stage_bytes(tn));
+__host__ __device__ constexpr int threads(bool gather) { return 192 + (gather ? 32 * HELPERS : 0); }
+__host__ __device__ constexpr int xbox(int tn) { return tn < 128 ? 16 : 32; }  // activation rows per TMA box
+// 128-byte K sub-blocks per ring slot (pairs: two, as in gemm_i8.cuh), rows of the
+// activation tile each CTA holds, bytes of a slot, ring depth.
+__host__ __device__ constexpr int ksub(bool pair) { return pair ? 2 : 1; }
+__host__ __device__ constexpr uint32_t x_bytes(int tn, bool pair) { return uint32_t(pair ? tn / 2 : tn) * BK; }
+__host__ __device__ constexpr uint32_t stage_bytes(int tn, bool pair) {
+  return uint32_t(ksub(pair)) * (W_BYTES + x_bytes(tn, pair));
 }
-__host__ __device__ constexpr uint32_t smem_bytes(int tn) { return uint32_t(stages(tn)) * stage_bytes(tn) + 1024; }
-__host__ __device__ constexpr int tmem_cols(int tn) { return 2 * tn < 32 ? 32 : 2 * tn; }
+__host__ __device__ constexpr int stages(int tn, bool pair) {
+  return int(198u * 1024u / stage_bytes(tn, pair)) > 10 ? 10 : int(198u * 1024u / stage_bytes(tn, pair));
+}
+__host__ __device__ constexpr uint32_t smem_bytes(int tn, bool pair) {
+  return uint32_t(stages(tn, pair)) * stage_bytes(tn, pair) + 4u * STAGE_OUT + 1024u;
+}
 }  // namespace grouped
 
 struct GroupedParams {
@@ -63,15 +77,25 @@ struct GroupedParams {
   void* out;        // [R, N] of OUT
 };
 
-// cp.async.bulk.tensor tile::gather4: four rows (row numbers r0..r3) of one
-// 128-byte column box to 512 bytes of shared memory.
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int4 r) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(r.x), "r"(r.y),
-      "r"(r.z), "r"(r.w)
-      : "memory");
+// cp.async.bulk.tensor tile::gather4: four rows (row numbers r) of one 128-byte
+// column box to 512 bytes of shared memory; completion on the mbarrier at
+// `mbar`, for PAIR a shared::cluster address that may be the peer CTA's.
+template <bool PAIR>
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* m, uint32_t mbar, int c0, int4 r) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(mbar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z),
+        "r"(r.w)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(mbar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z),
+        "r"(r.w)
+        : "memory");
 }
 
 // A named barrier that tells every thread whether all of them passed `ok`.
@@ -86,28 +110,30 @@ __device__ __forceinline__ bool named_barrier_and(int id, int nthreads, bool ok)
   return r != 0;
 }
 
-// One tile: expert, its weight row, its output rows.
+// One tile: expert, its first weight row (of the CTA or pair), its output rows.
 struct GroupedTile {
   int e, n0, r0, rows;  // rows <= TN
 };
 
-// The tiles of a CTA in order: a cursor over the prefix sums of tiles per expert.
-template <int TN>
+// The tiles of a unit in order: a cursor over the prefix sums of tiles per expert.
+// TN is a multiple of STEP, so every token tile but an expert's last is full and
+// the last is not empty.
+template <int TN, int TILE_N, int STEP>
 struct GroupedWalk {
   const int* cum;     // [E + 1] tiles before expert e
   const int* start;   // [E] first output row of expert e
   const int* count;   // [E] its rows
-  int E, n_tiles, e;
-  __device__ __forceinline__ GroupedWalk(const int* c, const int* s, const int* k, int E_, int nt)
-      : cum(c), start(s), count(k), E(E_), n_tiles(nt), e(0) {}
+  int E, e;
+  __device__ __forceinline__ GroupedWalk(const int* c, const int* s, const int* k, int E_)
+      : cum(c), start(s), count(k), E(E_), e(0) {}
   __device__ __forceinline__ GroupedTile at(int t) {
     while (e + 1 < E && t >= cum[e + 1]) ++e;
     const int local = t - cum[e];
     const int tok = (count[e] + TN - 1) / TN;       // token tiles of this expert
-    const int per = ((count[e] + tok - 1) / tok + 15) & ~15;
+    const int per = ((count[e] + tok - 1) / tok + STEP - 1) / STEP * STEP;
     GroupedTile g;
     g.e = e;
-    g.n0 = (local / tok) * grouped::BNW;
+    g.n0 = (local / tok) * TILE_N;
     const int j = (local % tok) * per;
     g.r0 = start[e] + j;
     g.rows = min(per, count[e] - j);
@@ -115,15 +141,26 @@ struct GroupedWalk {
   }
 };
 
-// TN: activation rows per tile at most (UMMA N); OUT: tg_dtype; GATHER: rows given.
-template <int TN, int OUT, bool GATHER>
-__global__ void __launch_bounds__(grouped::THREADS, 1)
+// TN: activation rows per tile at most (UMMA N); OUT: tg_dtype; GATHER: rows given;
+// PAIR: launched with clusters of 2 CTAs.
+template <int TN, int OUT, bool GATHER, bool PAIR>
+__global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     gemm_i8_grouped_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
-                           const GroupedParams p) {
+                           const __grid_constant__ CUtensorMap tma_out, const GroupedParams p) {
   using namespace grouped;
-  constexpr int S = stages(TN);
-  constexpr uint32_t STAGE = stage_bytes(TN);
-  constexpr uint32_t TMEM_COLS = tmem_cols(TN);
+  constexpr int S = stages(TN, PAIR);
+  constexpr int KS = ksub(PAIR);
+  constexpr uint32_t X_BYTES = x_bytes(TN, PAIR);
+  constexpr uint32_t STAGE = stage_bytes(TN, PAIR);
+  constexpr uint32_t TMEM_COLS = 2 * TN;
+  constexpr int STEP = PAIR ? 32 : 16;      // granularity of UMMA N
+  constexpr int TILE_N = PAIR ? 2 * BNW : BNW;
+  constexpr int XBOX = xbox(TN);
+  constexpr int THREADS = threads(GATHER);
+  constexpr int ESZ = OUT == 0 ? 4 : 2;
+  constexpr int CHUNK = 32 * 32 * ESZ;      // a staged chunk: 32 rows x 32 channels
+  constexpr int NBUF = STAGE_OUT / CHUNK;
+  static_assert(TN % 32 == 0 && 2 * TN >= 32 && 2 * TN <= 512, "token tile");
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -135,31 +172,41 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
   __shared__ __align__(8) uint64_t tempty_bar[2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_flag;
-  __shared__ int issued;  // ring slots the producer filled
+  __shared__ int issued;  // ring slots warp 0 filled
   __shared__ int cum[MAX_E + 1], start[MAX_E], count[MAX_E];
   __shared__ __align__(16) float col_xs[2][TN];
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
+  const int units = PAIR ? int(gridDim.x >> 1) : int(gridDim.x);
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tma_w);
     prefetch_tmap(&tma_x);
+    prefetch_tmap(&tma_out);
     for (int s = 0; s < S; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull_bar[b], 1);
-      mbar_init(&tempty_bar[b], 4);
+      mbar_init(&tempty_bar[b], PAIR ? 8 : 4);
     }
     fence_mbar_init();
     abort_flag = 0;
     issued = 0;
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base_sh, TMEM_COLS);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(&tmem_base_sh, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&tmem_base_sh, TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   // The offsets, xq and xscale are the previous kernel's.
   pdl_wait();
@@ -184,11 +231,11 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
     if (lane == 0) cum[0] = 0;
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync(); else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
   const int tiles = cum[p.E];
-  GroupedWalk<TN> walk(cum, start, count, p.E, p.n_tiles);
+  GroupedWalk<TN, TILE_N, STEP> walk(cum, start, count, p.E);
 
   // Bounded wait that also gives up as soon as another role has given up.
   auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int err) -> bool {
@@ -206,51 +253,71 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
     }
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
+  if (warp == 0 || warp >= 6) {
+    // ------------------------------------------------------------ producers
+    // Warp 0 loads the weight rows and announces the bytes.  Activation rows:
+    // by warp 0 in boxes, or gathered, each producer warp a quarter of them.
+    constexpr int XR = int(X_BYTES) / BK;             // activation rows of this CTA at most
+    constexpr int PRODUCERS = 1 + HELPERS;
+    constexpr int Q = (XR / 4 + PRODUCERS - 1) / PRODUCERS;  // gathers per warp at most
+    static_assert(Q <= 32, "one gather per lane");
+    const int part = warp == 0 ? 0 : warp - 5;
     int stage = 0, n_issued = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = unit; t < tiles && ok; t += units) {
       const GroupedTile g = walk.at(t);
-      const int nt = (g.rows + 15) & ~15;
-      // Lane l gathers rows 4 l .. 4 l + 3 of each 128; a row number outside
-      // xq reads row 0 (its scale is taken as 0).
-      constexpr int GL = (TN + 127) / 128;
-      int4 idx[GL];
-      if (GATHER) {
+      const int nt = (g.rows + STEP - 1) / STEP * STEP;
+      const int mine = PAIR ? nt / 2 : nt;            // activation rows this CTA loads
+      const int first = int(rank) * mine;             // the first of them in the tile
+      const int loaded = GATHER ? mine : (mine + XBOX - 1) / XBOX * XBOX;
+      const uint32_t tx = (PAIR ? 2u : 1u) * uint32_t(KS) * (W_BYTES + uint32_t(loaded) * BK);
+      // This lane's gather: rows 4 (part + PRODUCERS lane) + 0..3 of this CTA's.
+      // A row number outside xq reads row 0 (its scale is taken as 0).
+      const int gr = 4 * (part + PRODUCERS * lane);
+      int4 idx = make_int4(0, 0, 0, 0);
+      if (GATHER && gr < mine) {
+        int v[4];
 #pragma unroll
-        for (int i = 0; i < GL; ++i) {
-          int v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = i * 128 + lane * 4 + j;
-            v[j] = r < g.rows ? p.rows[g.r0 + r] : 0;
-            if (v[j] < 0 || v[j] >= p.M) v[j] = 0;
-          }
-          idx[i] = make_int4(v[0], v[1], v[2], v[3]);
+        for (int j = 0; j < 4; ++j) {
+          const int r = first + gr + j;
+          v[j] = r < g.rows ? p.rows[g.r0 + r] : 0;
+          if (v[j] < 0 || v[j] >= p.M) v[j] = 0;
         }
+        idx = make_int4(v[0], v[1], v[2], v[3]);
       }
-      const int wrow = g.e * p.N + g.n0;
+      const int wrow = g.e * p.N + g.n0 + int(rank) * BNW;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
         ok = __all_sync(0xffffffffu, wait(&empty_bar[stage], phase ^ 1u, DEVERR_PIPE_TIMEOUT));
         if (!ok) break;
         uint8_t* sw = smem + stage * STAGE;
-        uint8_t* sx = sw + W_BYTES;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full_bar[stage], W_BYTES + uint32_t(nt) * BK);
-          tma_load_2d(sw, &tma_w, &full_bar[stage], kb * BK, wrow);
+        uint8_t* sx = sw + KS * W_BYTES;
+        // Pairs: both CTAs' copies land on the even CTA's barrier, which expects
+        // the bytes of both.
+        const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full_bar[stage]), 0) : smem_u32(&full_bar[stage]);
+        if (warp == 0 && elect_one_lane()) {
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], tx);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const int kx = (kb * KS + ks) * BK;
+            if (PAIR) tma_load_2d_pair(sw + ks * W_BYTES, &tma_w, fb, kx, wrow);
+            else tma_load_2d(sw, &tma_w, &full_bar[stage], kx, wrow);
+            if (!GATHER) {
+              for (int r = 0; r < loaded; r += XBOX) {
+                uint8_t* dst = sx + ks * X_BYTES + r * BK;
+                if (PAIR) tma_load_2d_pair(dst, &tma_x, fb, kx, g.r0 + first + r);
+                else tma_load_2d(dst, &tma_x, &full_bar[stage], kx, g.r0 + first + r);
+              }
+            }
+          }
         }
         __syncwarp();
-        if (GATHER) {
+        if (GATHER && gr < mine) {
 #pragma unroll
-          for (int i = 0; i < GL; ++i) {
-            const int r = i * 128 + lane * 4;
-            if (r < nt) tma_gather4(sx + r * BK, &tma_x, &full_bar[stage], kb * BK, idx[i]);
-          }
-        } else if (lane * XBOX < nt) {
-          tma_load_2d(sx + lane * XBOX * BK, &tma_x, &full_bar[stage], kb * BK, g.r0 + lane * XBOX);
+          for (int ks = 0; ks < KS; ++ks)
+            tma_gather4<PAIR>(sx + ks * X_BYTES + gr * BK, &tma_x, fb, (kb * KS + ks) * BK, idx);
         }
+        __syncwarp();
         ++n_issued;
         if (++stage == S) {
           stage = 0;
@@ -258,16 +325,16 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
         }
       }
     }
-    if (lane == 0) issued = n_issued;
+    if (warp == 0 && lane == 0) issued = n_issued;
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    if (lane == 0 && leader) {
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++local) {
+      for (int t = unit; t < tiles && ok; t += units, ++local) {
         const GroupedTile g = walk.at(t);
-        const uint32_t idesc = gemm::idesc(BNW, (g.rows + 15) & ~15);
+        const uint32_t idesc = gemm::idesc(TILE_N, (g.rows + STEP - 1) / STEP * STEP);
         const int ab = local & 1;
         ok = wait(&tempty_bar[ab], (uint32_t(local >> 1) & 1u) ^ 1u, DEVERR_PIPE_TIMEOUT);
         if (!ok) break;
@@ -278,57 +345,86 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t w_addr = smem_u32(smem + stage * STAGE);
+          const uint32_t x_addr = w_addr + KS * W_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / UK; ++k)
-            mma_i8(d_tmem, gemm::kmajor_sw128_desc(w_addr + k * UK),
-                   gemm::kmajor_sw128_desc(w_addr + W_BYTES + k * UK), idesc, (kb | k) != 0 ? 1u : 0u);
-          mma_commit(&empty_bar[stage]);
+          for (int k = 0; k < KS * (BK / UK); ++k) {
+            const int ks = k / (BK / UK), kk = k % (BK / UK);
+            const uint64_t wd = gemm::kmajor_sw128_desc(w_addr + ks * W_BYTES + kk * UK);
+            const uint64_t xd = gemm::kmajor_sw128_desc(x_addr + ks * X_BYTES + kk * UK);
+            const uint32_t acc = (kb | k) != 0 ? 1u : 0u;
+            if (PAIR) mma_i8_pair(d_tmem, wd, xd, idesc, acc);
+            else mma_i8(d_tmem, wd, xd, idesc, acc);
+          }
+          if (PAIR) mma_commit_pair(&empty_bar[stage], 0x3); else mma_commit(&empty_bar[stage]);
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) mma_commit(&tfull_bar[ab]);
+        if (ok) {
+          if (PAIR) mma_commit_pair(&tfull_bar[ab], 0x3); else mma_commit(&tfull_bar[ab]);
+        }
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
     const int et = threadIdx.x - 64;  // 0..127
     const int quarter = warp & 3;     // TMEM lanes [32*quarter, +32)
-    int local = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++local) {
+    uint8_t* const sbufs = smem + S * STAGE + (warp - 2) * STAGE_OUT;
+    const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
+    const uint32_t tempty1 = PAIR ? mapa_shared(smem_u32(&tempty_bar[1]), 0) : 0u;
+    const bool hb = p.bias != nullptr;
+    int local = 0, chunk_seq = 0;  // chunk_seq: chunks this warp has staged, one bulk group each
+    for (int t = unit; t < tiles; t += units, ++local) {
       const GroupedTile g = walk.at(t);
       const int ab = local & 1;
-      const int n = g.n0 + quarter * 32 + lane;
+      const int n_warp = g.n0 + int(rank) * BNW + quarter * 32;
+      const int n = n_warp + lane;
       // This tile's row scales (two buffers: the warps may be a tile apart).
       for (int c = et; c < g.rows; c += 128) {
-        int a = GATHER ? p.rows[g.r0 + c] : g.r0 + c;
+        const int a = GATHER ? p.rows[g.r0 + c] : g.r0 + c;
         col_xs[ab][c] = a >= 0 && a < p.M ? p.xscale[a] : 0.0f;
       }
       float ws = 0.0f, bs = 0.0f;
       if (n < p.N) {
         const size_t en = size_t(g.e) * size_t(p.N) + size_t(n);
         ws = p.wscale[p.wscale_mode == 0 ? 0 : (p.wscale_mode == 1 ? size_t(g.e) : en)];
-        if (p.bias) bs = load_as_f32(p.bias, p.bias_dtype, en);
+        if (hb) bs = load_as_f32(p.bias, p.bias_dtype, en);
       }
-      const bool hb = p.bias != nullptr;
       // All four warps go on or none; the barrier also shows them the scales.
       if (!named_barrier_and(1, 128, wait(&tfull_bar[ab], uint32_t(local >> 1) & 1u, DEVERR_MMA_TIMEOUT))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(ab * TN);
-      const size_t esz = OUT == 0 ? 4 : 2;
-      char* o = static_cast<char*>(p.out) + (size_t(g.r0) * size_t(p.N) + size_t(n)) * esz;
 #pragma unroll 1
-      for (int c0 = 0; c0 < g.rows; c0 += 16) {
-        uint32_t acc[16];
-        tmem_ld_32x32b_x16(t_row + uint32_t(c0), acc);
+      for (int c0 = 0; c0 < g.rows; c0 += 32) {
+        uint32_t acc[32];
+        tmem_ld_32x32b_x32(t_row + uint32_t(c0), acc);
         tmem_wait_ld();
         reg_after_wait(acc);
-        if (n < p.N) {
+        if (c0 + 32 <= g.rows) {
+          uint8_t* const sbuf = sbufs + (chunk_seq % NBUF) * CHUNK;
+          ++chunk_seq;
+          // The store that last used this buffer must have finished reading it.
+          if (lane == 0) bulk_wait_read<NBUF - 1>();
+          __syncwarp();
+          char* o = reinterpret_cast<char*>(sbuf) + lane * ESZ;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < 32; ++j) {
+            if (hb) store_dequant<OUT, true>(o + j * 32 * ESZ, int32_t(acc[j]), col_xs[ab][c0 + j], ws, bs);
+            else store_dequant<OUT, false>(o + j * 32 * ESZ, int32_t(acc[j]), col_xs[ab][c0 + j], ws, bs);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (n_warp < p.N) tma_store_2d(&tma_out, sbuf, n_warp, g.r0 + c0);
+            bulk_commit();
+          }
+        } else if (n < p.N) {
+          char* o = static_cast<char*>(p.out) + (size_t(g.r0 + c0) * size_t(p.N) + size_t(n)) * ESZ;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
             if (c0 + j < g.rows) {
-              char* oj = o + size_t(c0 + j) * size_t(p.N) * esz;
+              char* oj = o + size_t(j) * size_t(p.N) * ESZ;
               if (hb) store_dequant<OUT, true>(oj, int32_t(acc[j]), col_xs[ab][c0 + j], ws, bs);
               else store_dequant<OUT, false>(oj, int32_t(acc[j]), col_xs[ab][c0 + j], ws, bs);
             }
@@ -338,22 +434,31 @@ __global__ void __launch_bounds__(grouped::THREADS, 1)
       // This warp is done reading the accumulator: hand it back to the MMA.
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty_bar[ab]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(ab ? tempty1 : tempty0);
+        else mbar_arrive(&tempty_bar[ab]);
+      }
     }
+    if (lane == 0) bulk_wait<0>();
   }
 
   __syncwarp();
-  tc_fence_before();
-  __syncthreads();
   // A wait gave up: let the loads still in flight (at most the last S slots)
-  // land before the CTA exits.
-  if (abort_flag && threadIdx.x == 0) {
+  // land before the CTA exits (pairs: they all land on the even CTA's barriers,
+  // and the odd one waits for it below).
+  if (abort_flag && threadIdx.x == 0 && leader) {
     for (int i = max(0, issued - S); i < issued; ++i)
       mbar_wait(&full_bar[i % S], uint32_t(i / S) & 1u, DEVERR_TMA_TIMEOUT);
   }
+  __syncwarp();
+  tc_fence_before();
+  // Neither CTA of a pair may leave while the other can still touch its shared
+  // memory or tensor memory.
+  if (PAIR) cluster_sync(); else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
