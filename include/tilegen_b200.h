@@ -265,7 +265,7 @@ int tg_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int to
                      float *weights, int32_t *ids, int32_t *offsets, int32_t *rows, int32_t *place, void *workspace,
                      size_t workspace_bytes, void *stream);
 
-/* Workspace bytes of tg_route_experts. */
+/* Workspace bytes of tg_route_experts (0 up to 256 tokens: then NULL will do). */
 size_t tg_route_experts_workspace(int64_t T, int64_t E);
 
 /*

@@ -1164,12 +1164,35 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
 // ------------------------------------------------------------ routed experts
 namespace {
 
-// Tokens per CTA of the router: a warp's eight tokens at most where the
-// tokens are few, more where the CTAs' counts would become many.
+// Tokens per CTA of the router's two-kernel form, a multiple of 32: a warp a
+// token and 32 warps, more where that would make more than 256 CTAs, whose
+// counts every CTA of the second kernel reads.
 int route_per_block(int64_t T) {
-  int64_t per = 32;
-  while ((T + per - 1) / per > 256) per += 32;
+  const int64_t per = (T + 256 * 32 - 1) / (256 * 32) * 32;
   return int(per);
+}
+
+template <int EPL>
+int launch_route(const tg::RouteParams& p, cudaStream_t st) {
+  const dim3 grid{unsigned(p.blocks)};
+  if (p.T <= tg::route::SINGLE)
+    return launch_dependent(tg::route_topk_kernel<EPL, false>, p, grid, tg::route::threads(EPL), 0, st);
+  const int rc = launch_dependent(tg::route_topk_kernel<EPL, true>, p, grid, tg::route::threads(EPL), 0, st);
+  if (rc != TG_OK) return rc;
+  return launch_dependent(tg::route_place_kernel, p, grid, tg::route::THREADS, 0, st);
+}
+
+template <int DT>
+int launch_combine(tg::CombineParams p, cudaStream_t st) {
+  constexpr int ESZ = DT == TG_DT_F32 ? 4 : 2;
+  constexpr int VEC = 16 / ESZ;
+  const bool vec = p.N % VEC == 0 && aligned16(p.y) && aligned16(p.residual) && aligned16(p.out);
+  p.per_row = uint32_t(vec ? p.N / VEC : p.N);
+  const int64_t ctas = (p.T * int64_t(p.per_row) + 255) / 256;
+  if (ctas > 0x7fffffff) return TG_ERR_UNSUPPORTED;
+  const dim3 grid{unsigned(ctas)};
+  return vec ? launch_dependent(tg::combine_kernel<DT, VEC>, p, grid, 256, 0, st)
+             : launch_dependent(tg::combine_kernel<DT, 1>, p, grid, 256, 0, st);
 }
 
 }  // namespace
@@ -1177,7 +1200,7 @@ int route_per_block(int64_t T) {
 extern "C" {
 
 size_t tg_route_experts_workspace(int64_t T, int64_t E) {
-  if (T <= 0 || E <= 0) return 0;
+  if (T <= tg::route::SINGLE || E <= 0) return 0;
   const int per = route_per_block(T);
   return size_t((T + per - 1) / per) * size_t(E) * 4;
 }
@@ -1192,11 +1215,12 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0)
     return cudaMemsetAsync(offsets, 0, size_t(E + 1) * 4, st) == cudaSuccess ? TG_OK : TG_ERR_CUDA;
-  if (!logits || !weights || !ids || !rows || !place || !workspace) return TG_ERR_INVALID_ARG;
+  const size_t need = tg_route_experts_workspace(T, E);
+  if (!logits || !weights || !ids || !rows || !place || (need > 0 && !workspace)) return TG_ERR_INVALID_ARG;
   if (!aligned_to(logits, dtype_bytes(dtype)) || !aligned_to(weights, 4) || !aligned_to(ids, 4) ||
       !aligned_to(rows, 4) || !aligned_to(place, 4) || !aligned_to(workspace, 4))
     return TG_ERR_MISALIGNED;
-  if (workspace_bytes < tg_route_experts_workspace(T, E)) return TG_ERR_INVALID_ARG;
+  if (workspace_bytes < need) return TG_ERR_INVALID_ARG;
   tg::RouteParams p;
   p.logits = logits;
   p.dtype = dtype;
@@ -1204,7 +1228,7 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
   p.E = int(E);
   p.top_k = top_k;
   p.renormalize = renormalize != 0;
-  p.per_block = route_per_block(T);
+  p.per_block = T <= tg::route::SINGLE ? tg::route::SINGLE : route_per_block(T);
   p.blocks = int((T + p.per_block - 1) / p.per_block);
   p.weights = weights;
   p.ids = ids;
@@ -1212,10 +1236,12 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
   p.rows = rows;
   p.place = place;
   p.counts = static_cast<int32_t*>(workspace);
-  const dim3 grid{unsigned(p.blocks)};
-  const int rc = launch_dependent(tg::route_topk_kernel, p, grid, tg::route::THREADS, 0, st);
-  if (rc != TG_OK) return rc;
-  return launch_dependent(tg::route_place_kernel, p, grid, tg::route::THREADS, 0, st);
+  if (E <= 32) return launch_route<1>(p, st);
+  if (E <= 64) return launch_route<2>(p, st);
+  if (E <= 128) return launch_route<4>(p, st);
+  if (E <= 256) return launch_route<8>(p, st);
+  if (E <= 512) return launch_route<16>(p, st);
+  return launch_route<32>(p, st);
 }
 
 int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place, const float* weights, int64_t T,
@@ -1240,11 +1266,10 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
   p.N = N;
   p.top_k = top_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid{unsigned(T)};
   switch (dtype) {
-    case TG_DT_F32: return launch_dependent(tg::combine_kernel<0>, p, grid, 256, 0, st);
-    case TG_DT_F16: return launch_dependent(tg::combine_kernel<1>, p, grid, 256, 0, st);
-    default: return launch_dependent(tg::combine_kernel<2>, p, grid, 256, 0, st);
+    case TG_DT_F32: return launch_combine<TG_DT_F32>(p, st);
+    case TG_DT_F16: return launch_combine<TG_DT_F16>(p, st);
+    default: return launch_combine<TG_DT_BF16>(p, st);
   }
 }
 
@@ -1253,32 +1278,31 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
 namespace {
 
 // The output's tensor map has to match the kernel's chunk (32 rows x 32 channels).
-template <int TN, int OUT, bool GATHER, bool PAIR>
+template <int TN, int OUT, bool GATHER>
 int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, tg::GroupedParams p, int dev,
                      int sms, cudaStream_t st) {
   static uint32_t attr_done[kMaxDevices];
   using namespace tg::grouped;
-  constexpr uint32_t smem = smem_bytes(TN, PAIR);
-  auto kern = tg::gemm_i8_grouped_kernel<TN, OUT, GATHER, PAIR>;
+  constexpr uint32_t smem = smem_bytes(TN);
+  auto kern = tg::gemm_i8_grouped_kernel<TN, OUT, GATHER>;
   if (!ensure_smem_attr(kern, dev, smem, attr_done)) return TG_ERR_CUDA;
-  constexpr int kTileN = PAIR ? 2 * BNW : BNW;
-  constexpr int64_t kKBlock = int64_t(BK) * ksub(PAIR);
-  p.n_tiles = int((int64_t(p.N) + kTileN - 1) / kTileN);
+  constexpr int64_t kKBlock = int64_t(BK) * KS;
+  p.n_tiles = int((int64_t(p.N) + TILE_N - 1) / TILE_N);
   p.k_blocks = int((int64_t(p.K) + kKBlock - 1) / kKBlock);
   // No more tiles than the full ones and a part-filled one for each expert.
   const int64_t most = (int64_t(p.R) / TN + std::min<int64_t>(p.E, p.R)) * p.n_tiles;
   // The pair GEMM's clusters of two take as much shared memory: as many fit.
-  const int units = int(std::min<int64_t>(gemm_units(dev, sms, PAIR), most));
+  const int units = int(std::min<int64_t>(std::max(gemm_units(dev, sms, true), 1), most));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(unsigned(PAIR ? 2 * units : units));
+  cfg.gridDim = dim3(unsigned(2 * units));
   cfg.blockDim = dim3(threads(GATHER));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -1287,21 +1311,21 @@ int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const CUtenso
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-template <int TN, bool PAIR>
+template <int TN>
 int launch_grouped_tn(const int8_t* xq, const CUtensorMap& tw, const CUtensorMap& to, const tg::GroupedParams& p,
                       int out_dtype, int dev, int sms, cudaStream_t st) {
   const bool g = p.rows != nullptr;
   CUtensorMap tx;
   if (!make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(p.K), uint64_t(p.M), uint64_t(p.K),
-                    tg::grouped::BK, g ? 1u : uint32_t(tg::grouped::xbox(TN)), CU_TENSOR_MAP_SWIZZLE_128B))
+                    tg::grouped::BK, g ? 1u : uint32_t(tg::grouped::XBOX), CU_TENSOR_MAP_SWIZZLE_128B))
     return TG_ERR_CUDA;
   switch (out_dtype) {
-    case TG_DT_F32: return g ? launch_grouped_t<TN, 0, true, PAIR>(tw, tx, to, p, dev, sms, st)
-                             : launch_grouped_t<TN, 0, false, PAIR>(tw, tx, to, p, dev, sms, st);
-    case TG_DT_F16: return g ? launch_grouped_t<TN, 1, true, PAIR>(tw, tx, to, p, dev, sms, st)
-                             : launch_grouped_t<TN, 1, false, PAIR>(tw, tx, to, p, dev, sms, st);
-    default: return g ? launch_grouped_t<TN, 2, true, PAIR>(tw, tx, to, p, dev, sms, st)
-                      : launch_grouped_t<TN, 2, false, PAIR>(tw, tx, to, p, dev, sms, st);
+    case TG_DT_F32: return g ? launch_grouped_t<TN, 0, true>(tw, tx, to, p, dev, sms, st)
+                             : launch_grouped_t<TN, 0, false>(tw, tx, to, p, dev, sms, st);
+    case TG_DT_F16: return g ? launch_grouped_t<TN, 1, true>(tw, tx, to, p, dev, sms, st)
+                             : launch_grouped_t<TN, 1, false>(tw, tx, to, p, dev, sms, st);
+    default: return g ? launch_grouped_t<TN, 2, true>(tw, tx, to, p, dev, sms, st)
+                      : launch_grouped_t<TN, 2, false>(tw, tx, to, p, dev, sms, st);
   }
 }
 
@@ -1358,9 +1382,9 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Rows an expert has on average, if every expert has some.
   const int64_t avg = R / std::min<int64_t>(E, R);
-  if (avg <= 24) return launch_grouped_tn<32, false>(xq, tw, to, p, out_dtype, dev, info.sms, st);
-  if (avg <= 128) return launch_grouped_tn<128, false>(xq, tw, to, p, out_dtype, dev, info.sms, st);
-  return launch_grouped_tn<256, true>(xq, tw, to, p, out_dtype, dev, info.sms, st);
+  if (avg <= 24) return launch_grouped_tn<64>(xq, tw, to, p, out_dtype, dev, info.sms, st);
+  if (avg <= 64) return launch_grouped_tn<128>(xq, tw, to, p, out_dtype, dev, info.sms, st);
+  return launch_grouped_tn<256>(xq, tw, to, p, out_dtype, dev, info.sms, st);
 }
 
 }  // extern "C"

@@ -11,6 +11,16 @@
 // The slots (t, j) that are left, in order of (expert, t, j), are the rows of the
 // grouped products: offsets[e] .. offsets[e+1] are expert e's, rows[r] is row
 // r's token, place[t,j] slot (t, j)'s row; rows behind offsets[E] are -1.
+//
+// A warp takes a token: lane l holds the logits l, l + 32, ... as order-preserving
+// 32-bit keys, and each of the top_k rounds is a maximum over the lane's keys
+// and two warp reductions (the key, then the lowest index that has it).  A token
+// has an expert at most once, so a CTA's slots of one expert are a bit mask over
+// its tokens: a slot's rank among them is a population count of the bits
+// before it, and no atomic's order decides anything.  Up to SINGLE tokens one CTA
+// does everything; above, a first kernel writes the choices and each CTA's
+// counts, a second one adds up the counts of the CTAs before it and places the
+// slots.  The launches and a few dependent memory latencies bound it.
 #pragma once
 
 #include "common.cuh"
@@ -19,17 +29,21 @@
 namespace tg {
 
 namespace route {
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
+constexpr int THREADS = 1024;                 // of the placing kernel
+// Of the choosing kernel: sixteen or more keys a lane leave 512 threads' registers.
+__host__ __device__ constexpr int threads(int epl) { return epl >= 16 ? 512 : 1024; }
 constexpr int MAX_E = TG_MAX_EXPERTS;
 constexpr int MAX_K = TG_MAX_TOP_K;
+constexpr int SINGLE = 256;                   // most tokens of the one-CTA form
+constexpr int MAX_WORDS = 8;                  // mask words of an expert in shared memory
+constexpr int PASS = 32 * MAX_WORDS;          // tokens whose masks are held at once
 }  // namespace route
 
 struct RouteParams {
   const void* logits;  // [T, E]
   int dtype;
   int T, E, top_k, renormalize;
-  int per_block;       // tokens per CTA
+  int per_block;       // tokens per CTA, a multiple of 32
   int blocks;          // ceil(T / per_block)
   float* weights;      // [T, top_k]
   int32_t* ids;        // [T, top_k]
@@ -46,130 +60,297 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+// The logit of a key (of NaN, a NaN).
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
 
-// The chosen experts and weights of every token, and each CTA's counts.
-// A warp per token; lane l holds the logits l, l + 32, ...
-__global__ void __launch_bounds__(route::THREADS) route_topk_kernel(const RouteParams p) {
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Token t's logits as keys: lane l's i-th is expert l + 32 i (0 past E).
+template <int EPL>
+__device__ __forceinline__ void route_load(const RouteParams& p, int t, int lane, uint32_t (&key)[EPL]) {
+  float v[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < p.E ? load_as_f32(p.logits, p.dtype, size_t(t) * p.E + e) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) key[i] = lane + 32 * i < p.E ? logit_key(v[i]) : 0u;
+}
+
+// The token's choices: lane j < top_k gets slot j's expert (-1: left out) and weight.
+template <int EPL>
+__device__ __forceinline__ void route_token(const RouteParams& p, int lane, uint32_t (&key)[EPL], int& id,
+                                            float& weight) {
+  id = -1;
+  uint32_t mine = 0;  // slot `lane`'s key
+  float all = 0.0f;   // sum over all experts, relative to the first choice
+  float top = 0.0f;
+  for (int j = 0; j < p.top_k; ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+    const uint32_t win = __reduce_max_sync(0xffffffffu, best);
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = EPL - 1; i >= 0; --i) at = key[i] == win ? lane + 32 * i : at;
+    const int e = EPL == 1 ? __ffs(__ballot_sync(0xffffffffu, key[0] == win)) - 1
+                           : int(__reduce_min_sync(0xffffffffu, at));
+    if (j == 0) {
+      const float v = key_logit(win);
+      top = v == -INFINITY ? 0.0f : v;
+      if (!p.renormalize) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) s += key[i] != 0u ? expf(key_logit(key[i]) - top) : 0.0f;
+        all = warp_sum(s);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (lane + 32 * i == e) key[i] = 0u;
+    if (lane == j) {
+      mine = win;
+      id = e;
+    }
+  }
+  const float v = key_logit(mine);
+  const float w = lane < p.top_k ? expf(v - top) : 0.0f;
+  if (p.renormalize) all = warp_sum(w);
+  const bool live = lane < p.top_k && v != -INFINITY;
+  if (!live) id = -1;
+  weight = live ? w / all : 0.0f;
+}
+
+// Exclusive prefix sum of total[0, E) into base (E + 1 values), by warp 0.
+__device__ __forceinline__ void route_scan(const int32_t* total, int32_t* base, int E, int lane) {
+  int sum = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    int v = e0 + lane < E ? total[e0 + lane] : 0;
+    const int own = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (e0 + lane < E) base[e0 + lane] = sum + v - own;
+    sum += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) base[E] = sum;
+}
+
+// MULTI: the choices and each CTA's counts only; otherwise (one CTA) everything.
+template <int EPL, bool MULTI>
+__global__ void __launch_bounds__(route::threads(EPL)) route_topk_kernel(const RouteParams p) {
   using namespace route;
-  __shared__ int32_t count[MAX_E];
+  constexpr int THREADS = threads(EPL);
+  constexpr int WARPS = THREADS / 32;
+  // MULTI counts with integer atomics; the one-CTA form keeps the masks.
+  __shared__ uint32_t mask[MULTI ? 1 : MAX_WORDS][MULTI ? 1 : EPL * 32];
+  __shared__ int32_t count[EPL * 32];
+  __shared__ int32_t base[MULTI ? 1 : EPL * 32 + 1];
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < p.E; e += THREADS) count[e] = 0;
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < p.E; e += THREADS) {
+    count[e] = 0;
+    if (!MULTI)
+      for (int w = 0; w < MAX_WORDS; ++w) mask[w][e] = 0u;
+  }
   __syncthreads();
   pdl_wait();
   const int t0 = blockIdx.x * p.per_block;
   const int t1 = min(t0 + p.per_block, p.T);
+  uint32_t key[EPL];
+  if (t0 + warp < t1) route_load<EPL>(p, t0 + warp, lane, key);
   for (int t = t0 + warp; t < t1; t += WARPS) {
-    uint32_t used = 0;  // bit i: logit lane + 32 i is taken
-    float top = 0.0f, sum = 0.0f, mine = 0.0f;
-    int id = -1;
-    for (int j = 0; j < p.top_k; ++j) {
-      uint32_t best = 0;
-      int at = 0x7fffffff;
-      for (int i = 0, e = lane; e < p.E; e += 32, ++i) {
-        if (used >> i & 1u) continue;
-        const uint32_t key = logit_key(load_as_f32(p.logits, p.dtype, size_t(t) * p.E + e));
-        if (key > best) {
-          best = key;
-          at = e;
-        }
-      }
-      const uint32_t win = __reduce_max_sync(0xffffffffu, best);
-      const int e = __reduce_min_sync(0xffffffffu, best == win ? at : 0x7fffffff);
-      if ((e & 31) == lane) used |= 1u << (e >> 5);
-      const float v = load_as_f32(p.logits, p.dtype, size_t(t) * p.E + e);
-      if (j == 0) top = v == -INFINITY ? 0.0f : v;
-      const float w = expf(v - top);
-      if (p.renormalize) sum += w;
-      if (lane == j) {
-        mine = w;
-        id = v == -INFINITY ? -1 : e;
-      }
-      if (lane == 0 && v != -INFINITY) atomicAdd(&count[e], 1);
-    }
-    if (!p.renormalize) {
-      for (int e = lane; e < p.E; e += 32) sum += expf(load_as_f32(p.logits, p.dtype, size_t(t) * p.E + e) - top);
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
+    uint32_t next[EPL];
+    if (t + WARPS < t1) route_load<EPL>(p, t + WARPS, lane, next);
+    int id;
+    float w;
+    route_token<EPL>(p, lane, key, id, w);
     if (lane < p.top_k) {
       p.ids[size_t(t) * p.top_k + lane] = id;
-      p.weights[size_t(t) * p.top_k + lane] = id < 0 ? 0.0f : mine / sum;
+      p.weights[size_t(t) * p.top_k + lane] = w;
+      if (id >= 0) {
+        if (MULTI) atomicAdd(&count[id], 1);
+        else atomicOr(&mask[(t - t0) >> 5][id], 1u << ((t - t0) & 31));
+      }
     }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = next[i];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += THREADS) p.counts[size_t(blockIdx.x) * p.E + e] = count[e];
+  if (MULTI) {
+    for (int e = threadIdx.x; e < p.E; e += THREADS) p.counts[size_t(blockIdx.x) * p.E + e] = count[e];
+    return;
+  }
+  for (int e = threadIdx.x; e < p.E; e += THREADS) {
+    int c = 0;
+    for (int w = 0; w < MAX_WORDS; ++w) c += __popc(mask[w][e]);
+    count[e] = c;
+  }
+  __syncthreads();
+  if (warp == 0) route_scan(count, base, p.E, lane);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= p.E; e += THREADS) p.offsets[e] = base[e];
+  const int slots = p.T * p.top_k;
+  for (int s = threadIdx.x; s < slots; s += THREADS) {
+    const int t = s / p.top_k;
+    const int e = p.ids[s];  // this CTA's own stores, behind the barriers above
+    int r = -1;
+    if (e >= 0) {
+      r = base[e] + __popc(mask[t >> 5][e] & ((1u << (t & 31)) - 1u));
+      for (int w = 0; w < (t >> 5); ++w) r += __popc(mask[w][e]);
+      p.rows[r] = t;
+    }
+    p.place[s] = r;
+    if (s >= base[p.E]) p.rows[s] = -1;
+  }
 }
 
 // The slots' rows.  Each CTA adds up the counts of the CTAs before it (and all
 // of them, for the offsets), then places its own slots in order.
 __global__ void __launch_bounds__(route::THREADS) route_place_kernel(const RouteParams p) {
   using namespace route;
-  __shared__ int32_t next[MAX_E];
-  __shared__ int32_t total[MAX_E];
+  __shared__ uint32_t mask[MAX_WORDS][MAX_E];
+  __shared__ int32_t before[MAX_E], total[MAX_E];
+  __shared__ int32_t base[MAX_E + 1];
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < p.E; e += THREADS) before[e] = total[e] = 0;
+  __syncthreads();
   pdl_wait();
-  for (int e = threadIdx.x; e < p.E; e += THREADS) {
-    int32_t before = 0, all = 0;
-    for (int b = 0; b < p.blocks; ++b) {
-      const int32_t c = p.counts[size_t(b) * p.E + e];
-      if (b < int(blockIdx.x)) before += c;
-      all += c;
+  // Neighbouring threads take neighbouring experts; the CTAs' counts are shared
+  // out over the groups of `span` threads.
+  const int span = min((p.E + 31) & ~31, THREADS);
+  const int groups = THREADS / span;
+  const int grp = threadIdx.x / span;
+  if (grp < groups) {
+    for (int e = threadIdx.x - grp * span; e < p.E; e += span) {
+      int32_t b = 0, a = 0;
+#pragma unroll 8
+      for (int i = grp; i < p.blocks; i += groups) {
+        const int32_t c = p.counts[size_t(i) * p.E + e];
+        a += c;
+        b += i < int(blockIdx.x) ? c : 0;
+      }
+      atomicAdd(&total[e], a);
+      atomicAdd(&before[e], b);
     }
-    next[e] = before;
-    total[e] = all;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int32_t sum = 0;
-    for (int e = 0; e < p.E; ++e) {
-      next[e] += sum;
-      if (blockIdx.x == 0) p.offsets[e] = sum;
-      sum += total[e];
-    }
-    if (blockIdx.x == 0) p.offsets[p.E] = sum;
-    total[0] = sum;
-  }
+  if (warp == 0) route_scan(total, base, p.E, lane);
   __syncthreads();
-  const int slots = p.T * p.top_k;
-  for (int r = total[0] + int(blockIdx.x * THREADS + threadIdx.x); r < slots; r += int(gridDim.x) * THREADS)
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= p.E; e += THREADS) p.offsets[e] = base[e];
+  const int live = base[p.E], slots = p.T * p.top_k;
+  for (int r = live + int(blockIdx.x * THREADS + threadIdx.x); r < slots; r += int(gridDim.x) * THREADS)
     p.rows[r] = -1;
-  if (threadIdx.x == 0) {
-    const int t0 = blockIdx.x * p.per_block;
-    const int t1 = min(t0 + p.per_block, p.T);
-    for (int s = t0 * p.top_k; s < t1 * p.top_k; ++s) {
-      const int e = p.ids[s];
-      const int r = e < 0 ? -1 : next[e]++;
+  const int t0 = blockIdx.x * p.per_block;
+  const int t1 = min(t0 + p.per_block, p.T);
+  for (int u0 = t0; u0 < t1; u0 += PASS) {  // PASS tokens at a time
+    const int u1 = min(u0 + PASS, t1);
+    const int words = (u1 - u0 + 31) >> 5;
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += THREADS)
+      for (int w = 0; w < words; ++w) mask[w][e] = 0u;
+    __syncthreads();
+    for (int s = u0 * p.top_k + threadIdx.x; s < u1 * p.top_k; s += THREADS) {
+      const int e = p.ids[s], u = s / p.top_k - u0;
+      if (e >= 0) atomicOr(&mask[u >> 5][e], 1u << (u & 31));
+    }
+    __syncthreads();
+    for (int s = u0 * p.top_k + threadIdx.x; s < u1 * p.top_k; s += THREADS) {
+      const int e = p.ids[s], t = s / p.top_k, u = t - u0;
+      int r = -1;
+      if (e >= 0) {
+        r = base[e] + before[e] + __popc(mask[u >> 5][e] & ((1u << (u & 31)) - 1u));
+        for (int w = 0; w < (u >> 5); ++w) r += __popc(mask[w][e]);
+        p.rows[r] = t;
+      }
       p.place[s] = r;
-      if (r >= 0) p.rows[r] = s / p.top_k;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += THREADS) {
+      int c = 0;
+      for (int w = 0; w < words; ++w) c += __popc(mask[w][e]);
+      before[e] += c;
     }
   }
 }
 
-// out[t,:] = (residual[t,:] +) sum_j weights[t,j] * y[place[t,j],:], in fp32, j
+// out[t,:] = sum_j weights[t,j] * y[place[t,j],:] (+ residual[t,:]), in fp32, j
 // ascending, rounded once.  A place outside [0, R) adds nothing.
 struct CombineParams {
   const void* y;          // [R, N] of DT
   const int32_t* place;   // [T, top_k]
   const float* weights;   // [T, top_k]
-  const void* residual;   // [T, N] of DT or NULL
+  const void* residual;   // [T, N] of DT or NULL; may be out
   void* out;              // [T, N] of DT
   int64_t R, T, N;
   int top_k;
+  uint32_t per_row;       // vectors (or elements) of a row
 };
 
-template <int DT>
+// VEC elements of a row per thread (16 bytes, or one where a row or an address
+// is not a multiple of 16 bytes).  One pass over the rows: HBM bound.  A
+// thread's loads of four slots are in flight together.
+template <int DT, int VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  constexpr int ESZ = DT == TG_DT_F32 ? 4 : 2;
+  pdl_launch_dependents();
   pdl_wait();
-  const int64_t t = blockIdx.x;
-  for (int64_t n = threadIdx.x; n < p.N; n += 256) {
-    float acc = 0.0f;
-    for (int j = 0; j < p.top_k; ++j) {
-      const int64_t r = p.place[t * p.top_k + j];
-      if (r < 0 || r >= p.R) continue;
-      acc = fmaf(p.weights[t * p.top_k + j], load_as_f32(p.y, DT, size_t(r) * p.N + n), acc);
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  // A 32-bit division wherever the index fits.
+  const int64_t t = (i >> 32) == 0 ? int64_t(uint32_t(i) / p.per_row) : i / int64_t(p.per_row);
+  if (t >= p.T) return;
+  const int64_t n = (i - t * p.per_row) * VEC;
+  float acc[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+  struct __align__(VEC * ESZ) Raw {
+    char b[VEC * ESZ];
+  };
+  auto add = [&](const Raw& raw, float w) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) acc[v] = fmaf(w, load_as_f32(&raw, DT, v), acc[v]);
+  };
+  const int32_t* place = p.place + t * p.top_k;
+  const float* weight = p.weights + t * p.top_k;
+  for (int j0 = 0; j0 < p.top_k; j0 += 4) {
+    Raw raw[4];
+    float w[4];
+    bool ok[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = j0 + j < p.top_k ? place[j0 + j] : -1;
+      ok[j] = r >= 0 && r < p.R;
+      if (ok[j]) {
+        w[j] = weight[j0 + j];
+        raw[j] = *reinterpret_cast<const Raw*>(static_cast<const char*>(p.y) + (r * p.N + n) * ESZ);
+      }
     }
-    if (p.residual) acc += load_as_f32(p.residual, DT, size_t(t) * p.N + n);
-    store_f32_as(p.out, DT, size_t(t) * p.N + n, acc);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (ok[j]) add(raw[j], w[j]);
   }
+  const int64_t o = (t * p.N + n) * ESZ;
+  if (p.residual) {
+    const Raw raw = *reinterpret_cast<const Raw*>(static_cast<const char*>(p.residual) + o);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) acc[v] += load_as_f32(&raw, DT, v);
+  }
+  Raw res;
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) store_f32_as(&res, DT, v, acc[v]);
+  *reinterpret_cast<Raw*>(static_cast<char*>(p.out) + o) = res;
 }
 
 }  // namespace tg

@@ -8,23 +8,23 @@
 // tg_int8_gemm_dequant on that expert's weight.
 //
 // Structure (persistent, one CTA per SM; roles as in gemm_i8.cuh: warp 0 TMA
-// producer, warp 1 MMA issuer, warps 2-5 epilogue; with gathered rows warps 6-8
+// producer, warp 1 MMA issuer, warps 2-5 epilogue; with gathered rows warps 6-12
 // are producers too):
-//  * The operands swap roles, as in gemm_splitk.cuh: a 128-row tile of an
+//  * The operands swap roles, as in gemm_splitk.cuh: a 256-row tile of an
 //    expert's WEIGHT is the UMMA M operand and up to TN of its activation rows
-//    are UMMA N.  N is set per tile (a multiple of 16, of 32 for pairs), so a
-//    group of three rows costs a 16-column product and three rows' loads, not
-//    a 128-row tile's, and nothing of a neighbouring group is ever computed.
-//  * PAIR: two CTAs of a cluster take 256 weight rows by the pair MMA; each
-//    loads its 128 weight rows and half of the activation rows.
+//    are UMMA N.  N is set per tile (a multiple of 32), so a group of three rows
+//    costs a 32-column product and as many rows' loads, not a 128-row tile's.
+//  * The two CTAs of a cluster share a tile by the pair MMA: each loads its
+//    128 weight rows and half of the activation rows.
 //  * The offsets stay on the device: each CTA turns them into a prefix sum of
 //    tiles per expert in shared memory, and its roles walk the tiles unit,
-//    unit + units, ... by it.  An expert's rows are cut into equal token tiles,
-//    which run fastest, so tiles in flight share their weight rows in L2; an
-//    expert without rows has no tile.
+//    unit + units, ... by it.  An expert's rows are cut into tiles of TN
+//    and a rest (a tile's loads, 256 + N rows, bound it as much as its product,
+//    so fewer tiles are cheaper than equal ones); these run fastest, so tiles in
+//    flight share their weight rows in L2.  An expert without rows has no tile.
 //  * Activation rows come by TMA, XBOX rows a box, or with `rows` by
 //    tile::gather4 (box one row high).  One lane issuing a gather takes about 50
-//    cycles, so four warps share them.
+//    cycles, so eight warps share them.
 //  * The epilogue holds one output channel per lane and a row per column: it
 //    stages 32 rows x 32 channels a warp in shared memory for one TMA store, and
 //    stores the part-filled last chunk of a group directly, row by row.
@@ -39,27 +39,25 @@
 namespace tg {
 
 namespace grouped {
-constexpr int BNW = 128;                 // weight rows per CTA (UMMA M per CTA)
+constexpr int BNW = 128;                 // weight rows per CTA
+constexpr int TILE_N = 2 * BNW;          // weight rows per pair (UMMA M)
+constexpr int STEP = 32;                 // granularity of the pair MMA's N
 constexpr int BK = 128;                  // bytes of K per k-block
 constexpr int UK = 32;                   // K per tcgen05.mma kind::i8
 constexpr uint32_t W_BYTES = BNW * BK;   // 16 KB
-constexpr int HELPERS = 3;               // producer warps beside warp 0 (gathered rows)
+constexpr int HELPERS = 7;               // producer warps beside warp 0 (gathered rows)
 constexpr int STAGE_OUT = 4096;          // epilogue staging bytes per warp
 constexpr int MAX_E = TG_MAX_EXPERTS;
 __host__ __device__ constexpr int threads(bool gather) { return 192 + (gather ? 32 * HELPERS : 0); }
-__host__ __device__ constexpr int xbox(int tn) { return tn < 128 ? 16 : 32; }  // activation rows per TMA box
-// 128-byte K sub-blocks per ring slot (pairs: two, as in gemm_i8.cuh), rows of the
-// activation tile each CTA holds, bytes of a slot, ring depth.
-__host__ __device__ constexpr int ksub(bool pair) { return pair ? 2 : 1; }
-__host__ __device__ constexpr uint32_t x_bytes(int tn, bool pair) { return uint32_t(pair ? tn / 2 : tn) * BK; }
-__host__ __device__ constexpr uint32_t stage_bytes(int tn, bool pair) {
-  return uint32_t(ksub(pair)) * (W_BYTES + x_bytes(tn, pair));
-}
-__host__ __device__ constexpr int stages(int tn, bool pair) {
-  return int(198u * 1024u / stage_bytes(tn, pair)) > 10 ? 10 : int(198u * 1024u / stage_bytes(tn, pair));
-}
-__host__ __device__ constexpr uint32_t smem_bytes(int tn, bool pair) {
-  return uint32_t(stages(tn, pair)) * stage_bytes(tn, pair) + 4u * STAGE_OUT + 1024u;
+constexpr int XBOX = 32;                 // activation rows per TMA box
+// 128-byte K sub-blocks per ring slot (two, as gemm_i8.cuh's pairs), bytes of a
+// sub-block's activation rows in each CTA (half of the tile's), of a slot, ring depth.
+constexpr int KS = 2;
+__host__ __device__ constexpr uint32_t x_bytes(int tn) { return uint32_t(tn / 2) * BK; }
+__host__ __device__ constexpr uint32_t stage_bytes(int tn) { return uint32_t(KS) * (W_BYTES + x_bytes(tn)); }
+__host__ __device__ constexpr int stages(int tn) { return int(198u * 1024u / stage_bytes(tn)); }
+__host__ __device__ constexpr uint32_t smem_bytes(int tn) {
+  return uint32_t(stages(tn)) * stage_bytes(tn) + 4u * STAGE_OUT + 1024u;
 }
 }  // namespace grouped
 
@@ -78,24 +76,15 @@ struct GroupedParams {
 };
 
 // cp.async.bulk.tensor tile::gather4: four rows (row numbers r) of one 128-byte
-// column box to 512 bytes of shared memory; completion on the mbarrier at
-// `mbar`, for PAIR a shared::cluster address that may be the peer CTA's.
-template <bool PAIR>
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* m, uint32_t mbar, int c0, int4 r) {
-  if (PAIR)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(mbar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z),
-        "r"(r.w)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(mbar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z),
-        "r"(r.w)
-        : "memory");
+// column box to 512 bytes of shared memory; completion on the mbarrier at the
+// shared::cluster address `mbar`, which may be the peer CTA's.
+__device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* m, uint32_t mbar, int c0, int4 r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(mbar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z),
+      "r"(r.w)
+      : "memory");
 }
 
 // A named barrier that tells every thread whether all of them passed `ok`.
@@ -116,9 +105,7 @@ struct GroupedTile {
 };
 
 // The tiles of a unit in order: a cursor over the prefix sums of tiles per expert.
-// TN is a multiple of STEP, so every token tile but an expert's last is full and
-// the last is not empty.
-template <int TN, int TILE_N, int STEP>
+template <int TN>
 struct GroupedWalk {
   const int* cum;     // [E + 1] tiles before expert e
   const int* start;   // [E] first output row of expert e
@@ -130,32 +117,27 @@ struct GroupedWalk {
     while (e + 1 < E && t >= cum[e + 1]) ++e;
     const int local = t - cum[e];
     const int tok = (count[e] + TN - 1) / TN;       // token tiles of this expert
-    const int per = ((count[e] + tok - 1) / tok + STEP - 1) / STEP * STEP;
     GroupedTile g;
     g.e = e;
-    g.n0 = (local / tok) * TILE_N;
-    const int j = (local % tok) * per;
+    g.n0 = (local / tok) * grouped::TILE_N;
+    const int j = (local % tok) * TN;
     g.r0 = start[e] + j;
-    g.rows = min(per, count[e] - j);
+    g.rows = min(TN, count[e] - j);
     return g;
   }
 };
 
-// TN: activation rows per tile at most (UMMA N); OUT: tg_dtype; GATHER: rows given;
-// PAIR: launched with clusters of 2 CTAs.
-template <int TN, int OUT, bool GATHER, bool PAIR>
+// TN: activation rows per tile at most (UMMA N); OUT: tg_dtype; GATHER: rows given.
+// Launched with clusters of 2 CTAs.
+template <int TN, int OUT, bool GATHER>
 __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     gemm_i8_grouped_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                            const __grid_constant__ CUtensorMap tma_out, const GroupedParams p) {
   using namespace grouped;
-  constexpr int S = stages(TN, PAIR);
-  constexpr int KS = ksub(PAIR);
-  constexpr uint32_t X_BYTES = x_bytes(TN, PAIR);
-  constexpr uint32_t STAGE = stage_bytes(TN, PAIR);
+  constexpr int S = stages(TN);
+  constexpr uint32_t X_BYTES = x_bytes(TN);
+  constexpr uint32_t STAGE = stage_bytes(TN);
   constexpr uint32_t TMEM_COLS = 2 * TN;
-  constexpr int STEP = PAIR ? 32 : 16;      // granularity of UMMA N
-  constexpr int TILE_N = PAIR ? 2 * BNW : BNW;
-  constexpr int XBOX = xbox(TN);
   constexpr int THREADS = threads(GATHER);
   constexpr int ESZ = OUT == 0 ? 4 : 2;
   constexpr int CHUNK = 32 * 32 * ESZ;      // a staged chunk: 32 rows x 32 channels
@@ -178,10 +160,10 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
-  const int units = PAIR ? int(gridDim.x >> 1) : int(gridDim.x);
+  const int unit = int(blockIdx.x >> 1);
+  const int units = int(gridDim.x >> 1);
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tma_w);
@@ -193,21 +175,18 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull_bar[b], 1);
-      mbar_init(&tempty_bar[b], PAIR ? 8 : 4);
+      mbar_init(&tempty_bar[b], 8);
     }
     fence_mbar_init();
     abort_flag = 0;
     issued = 0;
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(&tmem_base_sh, TMEM_COLS);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(&tmem_base_sh, TMEM_COLS);
-      tmem_relinquish();
-    }
+    tmem_alloc_pair(&tmem_base_sh, TMEM_COLS);
+    tmem_relinquish_pair();
   }
+  // The kernel after this one may start its prologue on SMs that are done here.
+  pdl_launch_dependents();
   // The offsets, xq and xscale are the previous kernel's.
   pdl_wait();
   for (int e = threadIdx.x; e < p.E; e += THREADS) {
@@ -231,11 +210,11 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     if (lane == 0) cum[0] = 0;
   }
   tc_fence_before();
-  if (PAIR) cluster_sync(); else __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
   const int tiles = cum[p.E];
-  GroupedWalk<TN, TILE_N, STEP> walk(cum, start, count, p.E);
+  GroupedWalk<TN> walk(cum, start, count, p.E);
 
   // Bounded wait that also gives up as soon as another role has given up.
   auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int err) -> bool {
@@ -268,10 +247,10 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     for (int t = unit; t < tiles && ok; t += units) {
       const GroupedTile g = walk.at(t);
       const int nt = (g.rows + STEP - 1) / STEP * STEP;
-      const int mine = PAIR ? nt / 2 : nt;            // activation rows this CTA loads
+      const int mine = nt / 2;                        // activation rows this CTA loads
       const int first = int(rank) * mine;             // the first of them in the tile
       const int loaded = GATHER ? mine : (mine + XBOX - 1) / XBOX * XBOX;
-      const uint32_t tx = (PAIR ? 2u : 1u) * uint32_t(KS) * (W_BYTES + uint32_t(loaded) * BK);
+      const uint32_t tx = 2u * uint32_t(KS) * (W_BYTES + uint32_t(loaded) * BK);
       // This lane's gather: rows 4 (part + PRODUCERS lane) + 0..3 of this CTA's.
       // A row number outside xq reads row 0 (its scale is taken as 0).
       const int gr = 4 * (part + PRODUCERS * lane);
@@ -292,22 +271,18 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
         if (!ok) break;
         uint8_t* sw = smem + stage * STAGE;
         uint8_t* sx = sw + KS * W_BYTES;
-        // Pairs: both CTAs' copies land on the even CTA's barrier, which expects
+        // Both CTAs' copies land on the even CTA's barrier, which expects
         // the bytes of both.
-        const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full_bar[stage]), 0) : smem_u32(&full_bar[stage]);
+        const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), 0);
         if (warp == 0 && elect_one_lane()) {
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], tx);
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
             const int kx = (kb * KS + ks) * BK;
-            if (PAIR) tma_load_2d_pair(sw + ks * W_BYTES, &tma_w, fb, kx, wrow);
-            else tma_load_2d(sw, &tma_w, &full_bar[stage], kx, wrow);
+            tma_load_2d_pair(sw + ks * W_BYTES, &tma_w, fb, kx, wrow);
             if (!GATHER) {
-              for (int r = 0; r < loaded; r += XBOX) {
-                uint8_t* dst = sx + ks * X_BYTES + r * BK;
-                if (PAIR) tma_load_2d_pair(dst, &tma_x, fb, kx, g.r0 + first + r);
-                else tma_load_2d(dst, &tma_x, &full_bar[stage], kx, g.r0 + first + r);
-              }
+              for (int r = 0; r < loaded; r += XBOX)
+                tma_load_2d_pair(sx + ks * X_BYTES + r * BK, &tma_x, fb, kx, g.r0 + first + r);
             }
           }
         }
@@ -315,7 +290,7 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
         if (GATHER && gr < mine) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
-            tma_gather4<PAIR>(sx + ks * X_BYTES + gr * BK, &tma_x, fb, (kb * KS + ks) * BK, idx);
+            tma_gather4_pair(sx + ks * X_BYTES + gr * BK, &tma_x, fb, (kb * KS + ks) * BK, idx);
         }
         __syncwarp();
         ++n_issued;
@@ -352,18 +327,15 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
             const uint64_t wd = gemm::kmajor_sw128_desc(w_addr + ks * W_BYTES + kk * UK);
             const uint64_t xd = gemm::kmajor_sw128_desc(x_addr + ks * X_BYTES + kk * UK);
             const uint32_t acc = (kb | k) != 0 ? 1u : 0u;
-            if (PAIR) mma_i8_pair(d_tmem, wd, xd, idesc, acc);
-            else mma_i8(d_tmem, wd, xd, idesc, acc);
+            mma_i8_pair(d_tmem, wd, xd, idesc, acc);
           }
-          if (PAIR) mma_commit_pair(&empty_bar[stage], 0x3); else mma_commit(&empty_bar[stage]);
+          mma_commit_pair(&empty_bar[stage], 0x3);
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) {
-          if (PAIR) mma_commit_pair(&tfull_bar[ab], 0x3); else mma_commit(&tfull_bar[ab]);
-        }
+        if (ok) mma_commit_pair(&tfull_bar[ab], 0x3);
       }
     }
   } else {
@@ -371,8 +343,8 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     const int et = threadIdx.x - 64;  // 0..127
     const int quarter = warp & 3;     // TMEM lanes [32*quarter, +32)
     uint8_t* const sbufs = smem + S * STAGE + (warp - 2) * STAGE_OUT;
-    const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(&tempty_bar[0]), 0) : 0u;
-    const uint32_t tempty1 = PAIR ? mapa_shared(smem_u32(&tempty_bar[1]), 0) : 0u;
+    const uint32_t tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    const uint32_t tempty1 = mapa_shared(smem_u32(&tempty_bar[1]), 0);
     const bool hb = p.bias != nullptr;
     int local = 0, chunk_seq = 0;  // chunk_seq: chunks this warp has staged, one bulk group each
     for (int t = unit; t < tiles; t += units, ++local) {
@@ -434,18 +406,15 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
       // This warp is done reading the accumulator: hand it back to the MMA.
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (PAIR) mbar_arrive_cluster(ab ? tempty1 : tempty0);
-        else mbar_arrive(&tempty_bar[ab]);
-      }
+      if (lane == 0) mbar_arrive_cluster(ab ? tempty1 : tempty0);
     }
     if (lane == 0) bulk_wait<0>();
   }
 
   __syncwarp();
   // A wait gave up: let the loads still in flight (at most the last S slots)
-  // land before the CTA exits (pairs: they all land on the even CTA's barriers,
-  // and the odd one waits for it below).
+  // land before the CTA exits (they all land on the even CTA's barriers, and the
+  // odd one waits for it below).
   if (abort_flag && threadIdx.x == 0 && leader) {
     for (int i = max(0, issued - S); i < issued; ++i)
       mbar_wait(&full_bar[i % S], uint32_t(i / S) & 1u, DEVERR_TMA_TIMEOUT);
@@ -454,11 +423,10 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
   tc_fence_before();
   // Neither CTA of a pair may leave while the other can still touch its shared
   // memory or tensor memory.
-  if (PAIR) cluster_sync(); else __syncthreads();
+  cluster_sync();
   if (warp == 1) {
     tc_fence_after();
-    if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
-    else tmem_dealloc(tmem_base, TMEM_COLS);
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
   }
 }
 
