@@ -151,11 +151,12 @@ def _route(logits=P, dt=0, t=4, e=8, k=2, w=P, ids=P, offsets=P, rows=P, place=P
 @pytest.mark.parametrize("kwargs,status", [
     ({"t": -1}, ARG), ({"e": 0}, ARG), ({"k": 0}, ARG), ({"k": 9}, ARG), ({"dt": 4}, ARG), ({"e": 1025}, UNS),
     ({"e": 64, "k": 33}, UNS), ({"t": 1 << 30}, UNS), ({"offsets": None}, ARG), ({"logits": None}, ARG), ({"w": None}, ARG),
-    ({"ids": None}, ARG), ({"rows": None}, ARG), ({"place": None}, ARG), ({"ws": None}, ARG), ({"bytes": 31}, ARG),
+    ({"ids": None}, ARG), ({"rows": None}, ARG), ({"place": None}, ARG), ({"t": 257, "ws": None}, ARG), ({"t": 257, "bytes": 31}, ARG), ({"t": 257, "ws": ctypes.c_void_p(258)}, MIS),
     ({"logits": ctypes.c_void_p(258)}, MIS), ({"place": ctypes.c_void_p(258)}, MIS), ({"offsets": ctypes.c_void_p(258)}, MIS),
 ])
 def test_route_entry_checks(kwargs, status):
-    assert _lib.lib().tg_route_experts_workspace(4, 8) >= 32
+    assert _lib.lib().tg_route_experts_workspace(257, 8) >= 9 * 8 * 4  # nine CTAs' counts
+    assert _lib.lib().tg_route_experts_workspace(256, 8) == 0
     assert _lib.lib().tg_route_experts_workspace(0, 8) == 0
     assert _route(**kwargs) == status
 

@@ -55,16 +55,24 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+# The current stream's handle on a device, without making a Stream object (1.2 us
+# of a call's ~10) where torch has the accessor its own generated code uses.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
 def _call(func: str, dev: torch.device, *args) -> None:
     L = _lib.lib()
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    stream = torch.cuda.current_stream(idx).cuda_stream
-    if idx != torch.cuda.current_device():
+    current = torch.cuda.current_device()
+    idx = dev.index if dev.index is not None else current
+    stream = _raw_stream(idx)
+    if idx != current:
         with torch.cuda.device(idx):
             st = getattr(L, func)(*args, stream)
     else:
         st = getattr(L, func)(*args, stream)
-    _lib.check(func, st)
+    if st:
+        _lib.check(func, st)
 
 
 def rotate_quant_max_k() -> int:
@@ -325,23 +333,24 @@ MAX_TOP_K = 32
 
 def _on(fn: str, name: str, t, dev: torch.device, dtypes, ndim: int) -> None:
     """``t`` is a tensor on ``dev`` of one of ``dtypes`` and of ``ndim`` dimensions, or ValueError."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.ndim == ndim and t.device == dev:
+        return
     if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f"{fn}: {name} must be a tensor on {dev}")
-    if t.dtype not in dtypes or t.ndim != ndim:
-        raise ValueError(f"{fn}: {name} must be {ndim}-D of {' / '.join(map(str, dtypes))}, got {tuple(t.shape)} "
-                         f"{t.dtype}")
+    raise ValueError(f"{fn}: {name} must be {ndim}-D of {' / '.join(map(str, dtypes))}, got {tuple(t.shape)} {t.dtype}")
 
 
 def _no_grad(fn: str, *tensors) -> None:
     """The forms for serving have no backward pass: an input that wants a gradient is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{fn}: no gradient is computed; call it under torch.no_grad() or on detached tensors")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{fn}: no gradient is computed; call it under torch.no_grad() or on detached tensors")
 
 
 def _out(fn: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, dev: torch.device,
          align: int = 16) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return torch.empty(*shape, dtype=dtype, device=dev)
     if (tuple(out.shape) != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous()
             or out.data_ptr() % align):
         raise ValueError(f"{fn}: out must be a contiguous {align}-byte aligned {list(shape)} {dtype} tensor on {dev}")
@@ -349,6 +358,7 @@ def _out(fn: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch
 
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_F32, _I8, _U8, _I32 = (torch.float32,), (torch.int8,), (torch.uint8,), (torch.int32,)
 
 
 def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor,
@@ -368,9 +378,9 @@ def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, 
     if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
         raise ValueError(f"{fn}: CUDA tensors required")
     dev = xq.device
-    _on(fn, "xq", xq, dev, (torch.int8,), 2)
-    _on(fn, "xscale", xscale, dev, (torch.float32,), 1)
-    _on(fn, "w4", w4, dev, (torch.uint8,), 2)
+    _on(fn, "xq", xq, dev, _I8, 2)
+    _on(fn, "xscale", xscale, dev, _F32, 1)
+    _on(fn, "w4", w4, dev, _U8, 2)
     _on(fn, "wscale", wscale, dev, _FLOATS, 2)
     if out_dtype not in _DTYPE_CODE:
         raise ValueError(f"{fn}: unsupported out_dtype {out_dtype}")
@@ -436,16 +446,16 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
         raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
     _no_grad(fn, logits)
     logits = logits.contiguous()
-    weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    offsets = torch.empty((e + 1,), dtype=torch.int32, device=dev)
-    rows = torch.empty((t * top_k,), dtype=torch.int32, device=dev)
-    place = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    need = int(_lib.lib().tg_route_experts_workspace(t, e))
-    work = torch.empty((need,), dtype=torch.uint8, device=dev)
-    _call("tg_route_experts", dev, logits.data_ptr(), _DTYPE_CODE[logits.dtype], t, e, top_k, int(bool(renormalize)),
-          weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), place.data_ptr(), work.data_ptr(),
-          need)
+    ids = torch.empty(t, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty_like(ids, dtype=torch.float32)
+    place = torch.empty_like(ids)
+    offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
+    rows = torch.empty(t * top_k, dtype=torch.int32, device=dev)
+    need = _lib.lib().tg_route_experts_workspace(t, e)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call("tg_route_experts", dev, logits.data_ptr(), _DTYPE_CODE[logits.dtype], t, e, top_k, 1 if renormalize else 0,
+          weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), place.data_ptr(),
+          work.data_ptr() if need else None, need)
     return ExpertRoutes(weights, ids, offsets, rows, place)
 
 
@@ -468,10 +478,10 @@ def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.
     if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
         raise ValueError(f"{fn}: CUDA tensors required")
     dev = xq.device
-    _on(fn, "xq", xq, dev, (torch.int8,), 2)
-    _on(fn, "xscale", xscale, dev, (torch.float32,), 1)
-    _on(fn, "wq", wq, dev, (torch.int8,), 3)
-    _on(fn, "offsets", offsets, dev, (torch.int32,), 1)
+    _on(fn, "xq", xq, dev, _I8, 2)
+    _on(fn, "xscale", xscale, dev, _F32, 1)
+    _on(fn, "wq", wq, dev, _I8, 3)
+    _on(fn, "offsets", offsets, dev, _I32, 1)
     if out_dtype not in _DTYPE_CODE:
         raise ValueError(f"{fn}: unsupported out_dtype {out_dtype}")
     m, k = xq.shape
@@ -496,7 +506,7 @@ def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.
         b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
     r, r_ptr = m, None
     if rows is not None:
-        _on(fn, "rows", rows, dev, (torch.int32,), 1)
+        _on(fn, "rows", rows, dev, _I32, 1)
         rows = rows.contiguous()
         r, r_ptr = rows.shape[0], rows.data_ptr()
     _no_grad(fn, xscale, wscale, bias)
@@ -525,8 +535,8 @@ def combine_experts(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor,
         raise ValueError(f"{fn}: CUDA tensors required")
     dev = y.device
     _on(fn, "y", y, dev, _FLOATS, 2)
-    _on(fn, "place", place, dev, (torch.int32,), 2)
-    _on(fn, "weights", weights, dev, (torch.float32,), 2)
+    _on(fn, "place", place, dev, _I32, 2)
+    _on(fn, "weights", weights, dev, _F32, 2)
     r, n = y.shape
     t, top_k = place.shape
     if weights.shape != place.shape or not 1 <= top_k <= MAX_TOP_K:
