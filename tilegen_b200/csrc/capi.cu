@@ -1094,23 +1094,31 @@ int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, 
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-template <int MT, int RT, int SV, bool S4>
+template <int MT, int RT, int WK, int SV, bool S4>
 int launch_gemv4_t(const tg::GemvI4Params& p, int dev, cudaStream_t st) {
   static uint32_t attr_done[kMaxDevices];
-  auto kern = tg::gemv_i4_kernel<MT, RT, SV, S4>;
-  constexpr uint32_t smem = tg::gemv4::smem_bytes(MT, RT);
-  if (!ensure_smem_attr(kern, dev, smem, attr_done)) return TG_ERR_CUDA;
-  return launch_dependent(kern, p, dim3(unsigned((int64_t(p.N) + RT * 16 - 1) / (RT * 16))), tg::gemv4::THREADS, smem, st);
+  auto kern = tg::gemv_i4_kernel<MT, RT, WK, SV, S4>;
+  if (!ensure_smem_attr(kern, dev, tg::gemv4::smem_bytes(8 * MT, MT, RT, WK), attr_done)) return TG_ERR_CUDA;
+  return launch_dependent(kern, p, dim3(unsigned((int64_t(p.N) + RT * 16 - 1) / (RT * 16))), WK * 32,
+                          tg::gemv4::smem_bytes(p.M, MT, RT, WK), st);
 }
 
 // sv: scales per block of 128 codes.
-template <int MT, int RT>
+template <int MT, int RT, int WK>
 int launch_gemv4_s(const tg::GemvI4Params& p, int sv, bool s4, int dev, cudaStream_t st) {
   switch (sv) {
-    case 4: return s4 ? launch_gemv4_t<MT, RT, 4, true>(p, dev, st) : launch_gemv4_t<MT, RT, 4, false>(p, dev, st);
-    case 2: return s4 ? launch_gemv4_t<MT, RT, 2, true>(p, dev, st) : launch_gemv4_t<MT, RT, 2, false>(p, dev, st);
-    default: return s4 ? launch_gemv4_t<MT, RT, 1, true>(p, dev, st) : launch_gemv4_t<MT, RT, 1, false>(p, dev, st);
+    case 4: return s4 ? launch_gemv4_t<MT, RT, WK, 4, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 4, false>(p, dev, st);
+    case 2: return s4 ? launch_gemv4_t<MT, RT, WK, 2, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 2, false>(p, dev, st);
+    default: return s4 ? launch_gemv4_t<MT, RT, WK, 1, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 1, false>(p, dev, st);
   }
+}
+
+template <int WK>
+int launch_gemv4_m(const tg::GemvI4Params& p, int sv, bool s4, int dev, cudaStream_t st) {
+  if (p.M <= 8) return launch_gemv4_s<1, 1, WK>(p, sv, s4, dev, st);
+  if (p.M <= 16) return launch_gemv4_s<2, 2, WK>(p, sv, s4, dev, st);
+  if (p.M <= 32) return launch_gemv4_s<4, 2, WK>(p, sv, s4, dev, st);
+  return launch_gemv4_s<8, 2, WK>(p, sv, s4, dev, st);
 }
 
 }  // namespace
@@ -1124,7 +1132,8 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (!is_dtype(out_dtype) || !is_dtype(wscale_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
   if (group != 32 && group != 64 && group != 128 && group != 256) return TG_ERR_UNSUPPORTED;
   if (M > TG_INT4_MAX_M || K % 128 != 0 || K % group != 0) return TG_ERR_UNSUPPORTED;
-  if (N >= (int64_t(1) << 31) || K >= (int64_t(1) << 31)) return TG_ERR_UNSUPPORTED;
+  // (32 rows of the weight are addressed with 32 bits.)
+  if (N >= (int64_t(1) << 31) || K >= (int64_t(1) << 24)) return TG_ERR_UNSUPPORTED;
   if (M == 0) return TG_OK;
   if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(w4) || !aligned16(wscale)) return TG_ERR_MISALIGNED;
@@ -1153,10 +1162,7 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sv = group == 32 ? 4 : (group == 64 ? 2 : 1);
   const bool s4 = wscale_dtype == TG_DT_F32;
-  if (M <= 8) return launch_gemv4_s<1, 1>(p, sv, s4, dev, st);
-  if (M <= 16) return launch_gemv4_s<2, 2>(p, sv, s4, dev, st);
-  if (M <= 32) return launch_gemv4_s<4, 2>(p, sv, s4, dev, st);
-  return launch_gemv4_s<8, 2>(p, sv, s4, dev, st);
+  return N / 16 >= 4 * info.sms_all ? launch_gemv4_m<4>(p, sv, s4, dev, st) : launch_gemv4_m<8>(p, sv, s4, dev, st);
 }
 
 }  // extern "C"

@@ -24,15 +24,16 @@
 // unpacked weight written to shared memory.  The activations are the N operand,
 // 8 rows a product, from shared memory (row pitch = 32 mod 128 bytes, so a
 // half-warp's 8-byte reads of four rows meet no bank twice).
-//  * A CTA is eight warps over the same RT * 16 weight rows; warp w takes the
-//    blocks w, w + 8, ...: eight neighbouring blocks (512 bytes of each weight
-//    row) are in flight together, and the activations' next KC columns come in
-//    by cp.async while the present ones are used.
+//  * A CTA is WK warps over the same RT * 16 weight rows; warp w takes the blocks
+//    w, w + WK, ...: neighbouring blocks are in flight together, and the
+//    activations' next KC columns come in by cp.async while the present ones
+//    are used.
 //  * The int32 accumulators start at the bits of 1.5 * 2^23, so that the finished
 //    sum v is the fp32 number 1.5 * 2^23 + v (|v| <= 2^21): one paired
 //    subtraction and one paired fma per two outputs and group, no conversion.
-//  * The eight warps' fp32 sums are added in order at the end.  The order of all
-//    additions depends on K alone, so a row's bits do not depend on M.
+//  * The warps' fp32 sums are added in order at the end.  WK follows from N
+//    alone, so the order of all additions, and with it a row's bits, does not
+//    depend on M.
 #pragma once
 
 #include "common.cuh"
@@ -41,17 +42,19 @@
 namespace tg {
 
 namespace gemv4 {
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
-// Activation columns per buffer (two buffers), a multiple of the 1024 that the
-// eight warps take in a step.
-__host__ __device__ constexpr int kc(int mt) { return mt == 1 ? 2048 : 1024; }
-__host__ __device__ constexpr int pitch(int mt) { return kc(mt) + 32; }
-__host__ __device__ constexpr uint32_t buf_bytes(int mt) { return uint32_t(mt * 8 * pitch(mt)); }
-__host__ __device__ constexpr uint32_t red_bytes(int mt, int rt) { return uint32_t(WARPS * rt * 16 * mt * 8 * 4); }
-__host__ __device__ constexpr uint32_t smem_bytes(int mt, int rt) {
-  return 2 * buf_bytes(mt) > red_bytes(mt, rt) ? 2 * buf_bytes(mt) : red_bytes(mt, rt);
+// Activation columns per buffer (two buffers): PER steps of the WK warps' blocks.
+__host__ __device__ constexpr int per(int mt, int wk) { return mt == 1 && wk == 4 ? 2 : 1; }
+__host__ __device__ constexpr int kc(int mt, int wk) { return per(mt, wk) * wk * 128; }
+__host__ __device__ constexpr int pitch(int mt, int wk) { return kc(mt, wk) + 32; }
+// Shared memory for m activation rows (m <= 8 mt): the buffers, later the warps'
+// partial tiles.
+__host__ __device__ constexpr uint32_t smem_bytes(int m, int mt, int rt, int wk) {
+  return uint32_t(2 * m * pitch(mt, wk)) > uint32_t(wk * rt * 16 * mt * 8 * 4)
+             ? uint32_t(2 * m * pitch(mt, wk)) : uint32_t(wk * rt * 16 * mt * 8 * 4);
 }
+// CTAs per SM the registers are held to, and weight blocks a lane loads ahead.
+__host__ __device__ constexpr int ctas(int mt, int wk) { return mt == 1 ? (wk == 4 ? 7 : 3) : (mt == 2 ? 2 : 1); }
+__host__ __device__ constexpr int depth(int rt) { return rt == 1 ? 3 : 2; }
 }  // namespace gemv4
 
 struct GemvI4Params {
@@ -133,13 +136,15 @@ struct RawScale {
   }
 };
 
-// MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per CTA; SV: scales
-// per block of 128 codes (groups of 32: 4, 64: 2, 128 and 256: 1); S4: fp32 scales.
-template <int MT, int RT, int SV, bool S4>
-__global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Params p) {
+// MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per CTA; WK: warps
+// along K; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128 and 256:
+// 1); S4: fp32 scales.
+template <int MT, int RT, int WK, int SV, bool S4>
+__global__ void __launch_bounds__(WK * 32, gemv4::ctas(MT, WK)) gemv_i4_kernel(const GemvI4Params p) {
   using namespace gemv4;
-  constexpr int KC = kc(MT), PITCH = pitch(MT), PER = KC / 1024;  // PER: a warp's blocks per buffer
-  constexpr int DEPTH = RT == 1 ? 4 : 2;
+  constexpr int THREADS = WK * 32;
+  constexpr int KC = kc(MT, WK), PITCH = pitch(MT, WK), PER = per(MT, WK);
+  constexpr int DEPTH = depth(RT);
   constexpr int ROWS = RT * 16, COLS = MT * 8;
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
   extern __shared__ __align__(16) uint8_t smem4[];
@@ -148,8 +153,9 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
   const int g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * ROWS;
   const int blocks = p.K >> 7;
-  const int steps = (blocks + WARPS - 1) / WARPS;
+  const int steps = (blocks + WK - 1) / WK;
   const size_t row_bytes = size_t(p.K) >> 1;
+  const uint32_t buf_bytes = uint32_t(p.M * PITCH);
   pdl_launch_dependents();
   if (p.prefetch > 0 && lane < 4) {
     const int r = warp * 4 + lane;
@@ -157,11 +163,10 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
   }
   pdl_wait();
 
-  // Activation columns [c KC, c KC + KC) into buffer c & 1; rows from M up stay
-  // as they are (they only reach outputs that are not stored).
+  // Activation columns [c KC, c KC + KC) into buffer c & 1.
   auto fetch = [&](int c) {
     const int k0 = c * KC, width = min(KC, p.K - k0) >> 4;
-    const uint32_t dst = smem_u32(smem4) + uint32_t(c & 1) * buf_bytes(MT);
+    const uint32_t dst = smem_u32(smem4) + uint32_t(c & 1) * buf_bytes;
     for (int i = threadIdx.x; i < p.M * (KC / 16); i += THREADS) {
       const int m = i / (KC / 16), k = i % (KC / 16);
       if (k < width) cp_async16(dst + uint32_t(m * PITCH + k * 16), p.xq + size_t(m) * p.K + k0 + k * 16);
@@ -170,27 +175,29 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
   };
 
   // This lane's weight rows (clamped: the rows past N are computed and dropped).
-  const uint8_t* wrow[RT][2];
-  const char* srow[RT][2];
+  // As 32-bit offsets from the first row of the CTA (K is below 2^24).
+  const uint8_t* const wbase = p.w4 + size_t(n0) * row_bytes;
   constexpr int SSZ = S4 ? 4 : 2;
+  const char* const sbase = static_cast<const char*>(p.wscale) + size_t(n0) * size_t(p.groups) * SSZ;
+  uint32_t wrow[RT][2], srow[RT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int n = min(n0 + r * 16 + h * 8 + g, p.N - 1);
-      wrow[r][h] = p.w4 + size_t(n) * row_bytes + t * 16;
-      srow[r][h] = static_cast<const char*>(p.wscale) + size_t(n) * size_t(p.groups) * SSZ;
+      const uint32_t n = uint32_t(min(r * 16 + h * 8 + g, p.N - 1 - n0));
+      wrow[r][h] = n * uint32_t(row_bytes) + t * 16;
+      srow[r][h] = n * uint32_t(p.groups * SSZ);
     }
   int4 wbuf[DEPTH][RT][2];
   RawScale<SV, S4> sbuf[DEPTH][RT][2];
   auto load = [&](int slot, int step) {
-    const int b = min(step * WARPS + warp, blocks - 1);
+    const int b = min(step * WK + warp, blocks - 1);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        wbuf[slot][r][h] = ld_stream_v4(reinterpret_cast<const int4*>(wrow[r][h] + size_t(b) * 64));
-        sbuf[slot][r][h].load(srow[r][h] + size_t((b >> p.scale_shift) * SV) * SSZ);
+        wbuf[slot][r][h] = ld_stream_v4(reinterpret_cast<const int4*>(wbase + (wrow[r][h] + uint32_t(b) * 64u)));
+        sbuf[slot][r][h].load(sbase + (srow[r][h] + uint32_t(b >> p.scale_shift) * uint32_t(SV * SSZ)));
       }
   };
 #pragma unroll
@@ -198,6 +205,11 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
     if (d < steps) load(d, d);
   fetch(0);
 
+  // Activation row of this lane in each 8-row tile (clamped: the columns past M
+  // are computed and dropped).
+  uint32_t xrow[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xrow[i] = uint32_t(min(i * 8 + g, p.M - 1) * PITCH + warp * 128 + t * 8);
   float2 acc[RT][MT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -215,8 +227,8 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
         __syncthreads();  // this buffer is in, and nobody reads the other one any more
         if ((s / PER + 1) * KC < p.K) fetch(s / PER + 1);
       }
-      if (s * WARPS + warp < blocks) {
-        const uint8_t* xs = smem4 + ((s / PER) & 1) * buf_bytes(MT) + g * PITCH + ((s % PER) * WARPS + warp) * 128 + t * 8;
+      if (s * WK + warp < blocks) {
+        const uint8_t* xs = smem4 + ((s / PER) & 1) * buf_bytes + (s % PER) * (WK * 128);
         uint32_t lo[RT][2][4], hi[RT][2][4];
         float sc[RT][2][SV];
 #pragma unroll
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
         for (int i = 0; i < MT; ++i) {
           uint2 x[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(xs + i * 8 * PITCH + j * 32);
+          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(xs + xrow[i] + j * 32);
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -261,7 +273,7 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
     }
   }
 
-  // Eight partial tiles [warp][column][row] into shared memory, added in order.
+  // The warps' partial tiles [warp][column][row] into shared memory, added in order.
   __syncthreads();
   float* red = reinterpret_cast<float*>(smem4);
 #pragma unroll
@@ -281,7 +293,7 @@ __global__ void __launch_bounds__(gemv4::THREADS) gemv_i4_kernel(const GemvI4Par
     if (n >= p.N) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) v += red[(w * COLS + m) * ROWS + r];
+    for (int w = 0; w < WK; ++w) v += red[(w * COLS + m) * ROWS + r];
     v = v * 0.0625f * p.xscale[m];
     if (p.bias) v += load_as_f32(p.bias, p.bias_dtype, size_t(n));
     store_f32_as(p.out, p.out_dtype, size_t(m) * p.N + n, v);
