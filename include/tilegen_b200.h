@@ -224,10 +224,11 @@ int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
  *   out[m,n] = (sum_g wscale[n,g] * float(sum_{k in g} xq[m,k] * w4[n,k])) * xscale[m] + bias[n]
  *
  * The inner sums are exact (a group of 256: each half's), the outer one is fp32
- * in an order that depends on N and K only (a row's result does not depend on
- * the other rows or on M).
+ * in an order that depends on K only (a row's result does not depend on the
+ * other rows or on M).
  *
- *   xq      [M, K] int8, 16-B aligned; K % 128 == 0, K < 2^24
+ *   xq      [M, K] int8, 16-B aligned; K % 128 == 0, K at most
+ *           tg_rotate_quant_max_k()
  *   w4      [N, K/2] bytes, 16-B aligned: of each 128 codes of a row, byte
  *           16 t + 4 j + b (t, j, b = 0..3) holds code 32 j + 8 t + b in its low
  *           and code 32 j + 8 t + 4 + b in its high half, two's complement

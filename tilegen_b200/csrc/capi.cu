@@ -1094,31 +1094,62 @@ int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, 
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-template <int MT, int RT, int WK, int SV, bool S4>
-int launch_gemv4_t(const tg::GemvI4Params& p, int dev, cudaStream_t st) {
+// Shared memory of a launch with `stages` ring slots: the ring (or the partial
+// tiles) and the scales.
+uint32_t gemv4_smem(int mt, int rows, int groups, int stages) {
+  using namespace tg::gemv4;
+  const uint32_t ring = uint32_t(stages) * (w_bytes(rows) + x_bytes(mt));
+  const uint32_t scales = uint32_t(rows * scale_pitch(groups)) * 4u;
+  return std::max(ring + scales, uint32_t(WK * 8 * mt * rows) * 4u) + 1024u;  // 1024: alignment slack
+}
+
+// want: CTAs per SM to make room for; as many ring slots as then fit (two at least).
+template <int MT, int RT, int WR, int SV>
+int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int want, int dev, cudaStream_t st) {
+  using namespace tg::gemv4;
   static uint32_t attr_done[kMaxDevices];
-  auto kern = tg::gemv_i4_kernel<MT, RT, WK, SV, S4>;
-  if (!ensure_smem_attr(kern, dev, tg::gemv4::smem_bytes(8 * MT, MT, RT, WK), attr_done)) return TG_ERR_CUDA;
-  return launch_dependent(kern, p, dim3(unsigned((int64_t(p.N) + RT * 16 - 1) / (RT * 16))), WK * 32,
-                          tg::gemv4::smem_bytes(p.M, MT, RT, WK), st);
+  constexpr uint32_t kStatic = 512;  // barriers and the abort flag, rounded up
+  auto kern = tg::gemv_i4_kernel<MT, RT, WR, SV>;
+  if (!ensure_smem_attr(kern, dev, kSmemPerCtaMax - kStatic, attr_done)) return TG_ERR_CUDA;
+  constexpr int kRows = rows(RT, WR);
+  const int steps = (p.K / 128 + WK - 1) / WK;
+  int stages = std::min(MAX_STAGES, std::max(2, steps));
+  auto fits = [&](int s, int ctas) {
+    return uint64_t(ctas) * (gemv4_smem(MT, kRows, p.groups, s) + kStatic + 1024u) <= kSmemPerSm;
+  };
+  while (want > 1 && !fits(3, want)) --want;
+  while (stages > 2 && !fits(stages, want)) --stages;
+  if (!fits(stages, 1)) return TG_ERR_UNSUPPORTED;
+  p.stages = stages;
+  p.prefetch = std::min(stages, steps);
+  CUtensorMap tw, tx;
+  if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w4, uint64_t(p.K) / 2, uint64_t(p.N), uint64_t(p.K) / 2, 128,
+                    uint32_t(kRows), CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(p.K), uint64_t(p.M), uint64_t(p.K), 128,
+                    uint32_t(p.M), CU_TENSOR_MAP_SWIZZLE_128B))
+    return TG_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(unsigned((int64_t(p.N) + kRows - 1) / kRows));
+  cfg.blockDim = dim3(threads(WR));
+  cfg.dynamicSmemBytes = gemv4_smem(MT, kRows, p.groups, stages);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, tw, tx, p) != cudaSuccess) return TG_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-// sv: scales per block of 128 codes.
-template <int MT, int RT, int WK>
-int launch_gemv4_s(const tg::GemvI4Params& p, int sv, bool s4, int dev, cudaStream_t st) {
+template <int MT, int RT, int WR>
+int launch_gemv4(const int8_t* xq, const uint8_t* w4, const tg::GemvI4Params& p, int sv, int want, int dev,
+                 cudaStream_t st) {
   switch (sv) {
-    case 4: return s4 ? launch_gemv4_t<MT, RT, WK, 4, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 4, false>(p, dev, st);
-    case 2: return s4 ? launch_gemv4_t<MT, RT, WK, 2, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 2, false>(p, dev, st);
-    default: return s4 ? launch_gemv4_t<MT, RT, WK, 1, true>(p, dev, st) : launch_gemv4_t<MT, RT, WK, 1, false>(p, dev, st);
+    case 4: return launch_gemv4_t<MT, RT, WR, 4>(xq, w4, p, want, dev, st);
+    case 2: return launch_gemv4_t<MT, RT, WR, 2>(xq, w4, p, want, dev, st);
+    default: return launch_gemv4_t<MT, RT, WR, 1>(xq, w4, p, want, dev, st);
   }
-}
-
-template <int WK>
-int launch_gemv4_m(const tg::GemvI4Params& p, int sv, bool s4, int dev, cudaStream_t st) {
-  if (p.M <= 8) return launch_gemv4_s<1, 1, WK>(p, sv, s4, dev, st);
-  if (p.M <= 16) return launch_gemv4_s<2, 2, WK>(p, sv, s4, dev, st);
-  if (p.M <= 32) return launch_gemv4_s<4, 2, WK>(p, sv, s4, dev, st);
-  return launch_gemv4_s<8, 2, WK>(p, sv, s4, dev, st);
 }
 
 }  // namespace
@@ -1132,17 +1163,14 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (!is_dtype(out_dtype) || !is_dtype(wscale_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
   if (group != 32 && group != 64 && group != 128 && group != 256) return TG_ERR_UNSUPPORTED;
   if (M > TG_INT4_MAX_M || K % 128 != 0 || K % group != 0) return TG_ERR_UNSUPPORTED;
-  // (32 rows of the weight are addressed with 32 bits.)
-  if (N >= (int64_t(1) << 31) || K >= (int64_t(1) << 24)) return TG_ERR_UNSUPPORTED;
+  if (N >= (int64_t(1) << 31) || K > kRotQuantMaxK) return TG_ERR_UNSUPPORTED;
   if (M == 0) return TG_OK;
   if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(w4) || !aligned16(wscale)) return TG_ERR_MISALIGNED;
   if (!aligned_to(xscale, 4) || !aligned_to(out, dtype_bytes(out_dtype)) || (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
     return TG_ERR_MISALIGNED;
   tg::GemvI4Params p;
-  p.xq = xq;
   p.xscale = xscale;
-  p.w4 = w4;
   p.wscale = wscale;
   p.bias = bias;
   p.wscale_dtype = wscale_dtype;
@@ -1153,16 +1181,21 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   p.M = int(M);
   p.N = int(N);
   p.K = int(K);
-  // A quarter of each row, as the int8 GEMV.
-  p.prefetch = N * K / 2 <= kGemvPrefetchMaxBytes ? int(K / 8 / 16 * 16) : 0;
   p.out = out;
   int dev;
   DeviceInfo info;
   if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sv = group == 32 ? 4 : (group == 64 ? 2 : 1);
-  const bool s4 = wscale_dtype == TG_DT_F32;
-  return N / 16 >= 4 * info.sms_all ? launch_gemv4_m<4>(p, sv, s4, dev, st) : launch_gemv4_m<8>(p, sv, s4, dev, st);
+  // CTAs an SM would get if all ran at once.
+  const int64_t tiles = (N + 15) / 16;
+  const int want = int(std::max<int64_t>(1, std::min<int64_t>(7, (tiles + info.sms_all - 1) / info.sms_all)));
+  if (M <= 8) return launch_gemv4<1, 1, 1>(xq, w4, p, sv, want, dev, st);
+  if (M <= 16) return launch_gemv4<2, 2, 1>(xq, w4, p, sv, std::min(3, (want + 1) / 2), dev, st);
+  if (M <= 32) return launch_gemv4<4, 2, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
+  const int rc = launch_gemv4<8, 2, 2>(xq, w4, p, sv, 1, dev, st);
+  // Very long rows of fine scales leave no room for 64 rows of them.
+  return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1>(xq, w4, p, sv, 1, dev, st) : rc;
 }
 
 }  // extern "C"

@@ -16,51 +16,52 @@
 // (w << 4) & 0xf0f0f0f0 and w & 0xf0f0f0f0 are 16 times the codes (the sign bit
 // of the 4-bit code lands on the byte's); the factor 16 goes into the epilogue.
 //
-// What bounds it: the weight's bytes.  A row tile of 16 weights is the products'
-// M operand, straight from registers: each lane loads its 16 bytes of the rows
-// lane/4 and lane/4 + 8 (no shared memory for the weight), DEPTH blocks ahead.
-// The legacy mma.sync is enough here: at 64 rows the products are 20 % of its
-// measured 1140 TOP/s at the weight's HBM rate, while tcgen05 would need the
-// unpacked weight written to shared memory.  The activations are the N operand,
-// 8 rows a product, from shared memory (row pitch = 32 mod 128 bytes, so a
-// half-warp's 8-byte reads of four rows meet no bank twice).
-//  * A CTA is WK warps over the same RT * 16 weight rows; warp w takes the blocks
-//    w, w + WK, ...: neighbouring blocks are in flight together, and the
-//    activations' next KC columns come in by cp.async while the present ones
-//    are used.
+// What bounds it: the weight's bytes, while the rows are few.  The weight comes
+// through a ring of shared memory by TMA, which keeps tens of KB in flight per SM
+// without a register, and is the products' M operand (legacy mma.sync: at 64 rows
+// the products are 20 % of its measured 1140 TOP/s at the weight's HBM rate, and
+// tcgen05 would need the unpacked weight written back to shared memory); the
+// activations are the N operand, 8 rows a product.
+//  * A CTA has WR * RT * 16 weight rows and all of K.  A step is four blocks of 128
+//    codes, one for each of the four warps along K, so the activations of a step
+//    are read once per CTA.  The order of all additions depends on K alone: a
+//    row's bits depend neither on M nor on the other rows.
+//  * Both come in boxes of 128 bytes a row with the 128-byte swizzle (narrower
+//    rows, laid out for the reads, made the TMA unit the bound: it takes rows
+//    at a fixed rate).  A quad reads 64 bytes of a weight row and 32 of an
+//    activation row; lane g's row is picked (w_row, x_row) so that the rows one
+//    shared-memory pass reads lie in different banks.  Blocks past K and rows
+//    past N arrive as zeros, so the loop has no edges.
+//  * The rows' scales are put into shared memory as fp32 at the start.
 //  * The int32 accumulators start at the bits of 1.5 * 2^23, so that the finished
 //    sum v is the fp32 number 1.5 * 2^23 + v (|v| <= 2^21): one paired
 //    subtraction and one paired fma per two outputs and group, no conversion.
-//  * The warps' fp32 sums are added in order at the end.  WK follows from N
-//    alone, so the order of all additions, and with it a row's bits, does not
-//    depend on M.
 #pragma once
 
 #include "common.cuh"
-#include "gemv_i8.cuh"
 
 namespace tg {
 
 namespace gemv4 {
-// Activation columns per buffer (two buffers): PER steps of the WK warps' blocks.
-__host__ __device__ constexpr int per(int mt, int wk) { return mt == 1 && wk == 4 ? 2 : 1; }
-__host__ __device__ constexpr int kc(int mt, int wk) { return per(mt, wk) * wk * 128; }
-__host__ __device__ constexpr int pitch(int mt, int wk) { return kc(mt, wk) + 32; }
-// Shared memory for m activation rows (m <= 8 mt): the buffers, later the warps'
-// partial tiles.
-__host__ __device__ constexpr uint32_t smem_bytes(int m, int mt, int rt, int wk) {
-  return uint32_t(2 * m * pitch(mt, wk)) > uint32_t(wk * rt * 16 * mt * 8 * 4)
-             ? uint32_t(2 * m * pitch(mt, wk)) : uint32_t(wk * rt * 16 * mt * 8 * 4);
-}
-// CTAs per SM the registers are held to, and weight blocks a lane loads ahead.
-__host__ __device__ constexpr int ctas(int mt, int wk) { return mt == 1 ? (wk == 4 ? 7 : 3) : (mt == 2 ? 2 : 1); }
-__host__ __device__ constexpr int depth(int rt) { return rt == 1 ? 3 : 2; }
+constexpr int WK = 4;                 // warps along K = blocks of 128 codes per step
+constexpr int MAX_STAGES = 16;
+__host__ __device__ constexpr int threads(int wr) { return 32 * (WK * wr + 1); }
+__host__ __device__ constexpr int rows(int rt, int wr) { return 16 * rt * wr; }
+// Bytes of a ring slot's weights ([two blocks][row][128]) and activations
+// ([block][row][128]); words of a row's scales (eight rows start in different banks).
+__host__ __device__ constexpr uint32_t w_bytes(int rows) { return uint32_t(rows) * WK * 64; }
+__host__ __device__ constexpr uint32_t x_bytes(int mt) { return uint32_t(mt) * WK * 1024; }
+__host__ __device__ constexpr int scale_pitch(int groups) { return (groups + 16 + 31) / 32 * 32 + 4; }
+// The weight row and the activation row, of eight, that lanes 4 g .. 4 g + 3 hold.
+// Swizzled, byte chunk c of row r lies at c ^ r: a pass of eight lanes reads 64
+// bytes of w_row 2i and 2i + 1, which differ in bit 2 (other halves of the 128
+// bytes); a pass of sixteen reads 32 bytes of four x_rows, which differ in bits 1-2.
+__device__ __forceinline__ int w_row(int g) { return (g >> 1) | ((g & 1) << 2); }
+__device__ __forceinline__ int x_row(int g) { return ((g & 3) << 1) | (g >> 2); }
 }  // namespace gemv4
 
 struct GemvI4Params {
-  const int8_t* xq;
   const float* xscale;
-  const uint8_t* w4;
   const void* wscale;   // [N, groups] of wscale_dtype
   const void* bias;
   int wscale_dtype;
@@ -69,7 +70,8 @@ struct GemvI4Params {
   int groups;           // K / group
   int scale_shift;      // groups of 256: 1 (two blocks share a scale), else 0
   int M, N, K;
-  int prefetch;         // bytes of each weight row asked into L2 before the dependent wait
+  int stages;           // ring slots
+  int prefetch;         // slots' weights asked into L2 before the dependent wait
   void* out;            // [M, N] of out_dtype
 };
 
@@ -89,203 +91,249 @@ __device__ __forceinline__ void store_f32_as(void* out, int dtype, size_t i, flo
   else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(r);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// The scales of rows [n0, n0 + ROWS) to shared memory as fp32, `pitch` words a row,
+// by THREADS threads: one contiguous, 16-byte aligned stretch (n0 is a multiple
+// of 16), read 16 bytes at a time.  Zeros behind a row's last group, for the
+// blocks past K; the rows past N are dropped and left alone.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void stage_scales(const GemvI4Params& p, int n0, float* scale, int pitch) {
+  const bool f32 = p.wscale_dtype == TG_DT_F32, f16 = p.wscale_dtype == TG_DT_F16;
+  const int per = f32 ? 4 : 8;
+  const int valid = min(ROWS, p.N - n0) * p.groups;
+  const char* src = static_cast<const char*>(p.wscale) + size_t(n0) * size_t(p.groups) * (f32 ? 4 : 2);
+#pragma unroll 4
+  for (int i = threadIdx.x * per; i < valid; i += THREADS * per) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (i + per <= valid) {
+      v = *reinterpret_cast<const uint4*>(src + i * (16 / per));
+    } else {  // the last, part-filled 16 bytes of the tensor
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      for (int k = 0; i + k < valid; ++k) {
+        if (f32) w[k] = reinterpret_cast<const uint32_t*>(src)[i + k];
+        else w[k >> 1] |= uint32_t(reinterpret_cast<const unsigned short*>(src)[i + k]) << ((k & 1) * 16);
+      }
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    int r = i / p.groups, c = i - r * p.groups;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < per && i + k < valid) {
+        const uint32_t h = (k & 1) ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
+        scale[r * pitch + c] = f32 ? __uint_as_float(w[k & 3])
+                                   : (f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h)))
+                                          : __uint_as_float(h << 16));
+      }
+      if (++c == p.groups) {
+        c = 0;
+        ++r;
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < ROWS * 16; i += THREADS) scale[(i >> 4) * pitch + p.groups + (i & 15)] = 0.0f;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// d += a (16 x 32, rows) * b (32 x 8, columns), int8 -> int32.
-__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
+// d = a (16 x 32, rows) * b (32 x 8, columns) + c, int8 -> int32.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b,
+                                       const int (&c)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 
-// One block's scales of a row: SV of them (one per 128 / SV codes), as loaded.
-template <int SV, bool S4>
-struct RawScale {
-  uint32_t v[S4 ? SV : (SV + 1) / 2];
-  __device__ __forceinline__ void load(const void* p) {
-    constexpr int BYTES = SV * (S4 ? 4 : 2);
-    if constexpr (BYTES == 2) {
-      v[0] = __ldg(static_cast<const unsigned short*>(p));
-    } else if constexpr (BYTES == 4) {
-      v[0] = __ldg(static_cast<const uint32_t*>(p));
-    } else if constexpr (BYTES == 8) {
-      const uint2 a = __ldg(static_cast<const uint2*>(p));
-      v[0] = a.x;
-      v[1] = a.y;
-    } else {
-      const uint4 a = __ldg(static_cast<const uint4*>(p));
-      v[0] = a.x;
-      v[1] = a.y;
-      v[2] = a.z;
-      v[3] = a.w;
-    }
-  }
-  __device__ __forceinline__ float get(int i, bool f16) const {
-    if constexpr (S4) {
-      return __uint_as_float(v[i]);
-    } else {
-      const uint32_t h = (i & 1) ? v[i / 2] >> 16 : v[i / 2] & 0xffffu;
-      return f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16);
-    }
-  }
-};
-
-// MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per CTA; WK: warps
-// along K; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128 and 256:
-// 1); S4: fp32 scales.
-template <int MT, int RT, int WK, int SV, bool S4>
-__global__ void __launch_bounds__(WK * 32, gemv4::ctas(MT, WK)) gemv_i4_kernel(const GemvI4Params p) {
+// MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per warp; WR:
+// warps along N; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128
+// and 256: 1).
+template <int MT, int RT, int WR, int SV>
+__global__ void __launch_bounds__(gemv4::threads(WR))
+    gemv_i4_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
+                   const GemvI4Params p) {
   using namespace gemv4;
-  constexpr int THREADS = WK * 32;
-  constexpr int KC = kc(MT, WK), PITCH = pitch(MT, WK), PER = per(MT, WK);
-  constexpr int DEPTH = depth(RT);
-  constexpr int ROWS = RT * 16, COLS = MT * 8;
+  constexpr int THREADS = threads(WR);
+  constexpr int ROWS = rows(RT, WR), COLS = MT * 8;
+  constexpr uint32_t W_BYTES = w_bytes(ROWS);
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
-  extern __shared__ __align__(16) uint8_t smem4[];
+  // Ring slots [weights | activations], then the scales; the partial tiles of the
+  // end lie over the ring.
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem4 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+  __shared__ volatile int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * ROWS;
-  const int blocks = p.K >> 7;
-  const int steps = (blocks + WK - 1) / WK;
-  const size_t row_bytes = size_t(p.K) >> 1;
-  const uint32_t buf_bytes = uint32_t(p.M * PITCH);
+  const int steps = (p.K / 128 + WK - 1) / WK;
+  constexpr uint32_t SLOT = W_BYTES + x_bytes(MT);
+  const int pitch = scale_pitch(p.groups);
+  float* const scale = reinterpret_cast<float*>(smem4 + uint32_t(p.stages) * SLOT);
   pdl_launch_dependents();
-  if (p.prefetch > 0 && lane < 4) {
-    const int r = warp * 4 + lane;
-    if (r < ROWS && n0 + r < p.N) prefetch_l2_bulk(p.w4 + size_t(n0 + r) * row_bytes, uint32_t(p.prefetch));
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tma_w);
+    prefetch_tmap(&tma_x);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], WK * WR);
+    }
+    fence_mbar_init();
+    abort_flag = 0;
+    // Only into L2: the kernel before may be the one that wrote the weight.
+    for (int s = 0; s < 2 * p.prefetch; ++s) tma_prefetch_l2_2d(&tma_w, s * 128, n0);
   }
+  __syncthreads();
   pdl_wait();
 
-  // Activation columns [c KC, c KC + KC) into buffer c & 1.
-  auto fetch = [&](int c) {
-    const int k0 = c * KC, width = min(KC, p.K - k0) >> 4;
-    const uint32_t dst = smem_u32(smem4) + uint32_t(c & 1) * buf_bytes;
-    for (int i = threadIdx.x; i < p.M * (KC / 16); i += THREADS) {
-      const int m = i / (KC / 16), k = i % (KC / 16);
-      if (k < width) cp_async16(dst + uint32_t(m * PITCH + k * 16), p.xq + size_t(m) * p.K + k0 + k * 16);
-    }
-    cp_async_commit();
-  };
-
-  // This lane's weight rows (clamped: the rows past N are computed and dropped).
-  // As 32-bit offsets from the first row of the CTA (K is below 2^24).
-  const uint8_t* const wbase = p.w4 + size_t(n0) * row_bytes;
-  constexpr int SSZ = S4 ? 4 : 2;
-  const char* const sbase = static_cast<const char*>(p.wscale) + size_t(n0) * size_t(p.groups) * SSZ;
-  uint32_t wrow[RT][2], srow[RT][2];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t n = uint32_t(min(r * 16 + h * 8 + g, p.N - 1 - n0));
-      wrow[r][h] = n * uint32_t(row_bytes) + t * 16;
-      srow[r][h] = n * uint32_t(p.groups * SSZ);
-    }
-  int4 wbuf[DEPTH][RT][2];
-  RawScale<SV, S4> sbuf[DEPTH][RT][2];
-  auto load = [&](int slot, int step) {
-    const int b = min(step * WK + warp, blocks - 1);
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        wbuf[slot][r][h] = ld_stream_v4(reinterpret_cast<const int4*>(wbase + (wrow[r][h] + uint32_t(b) * 64u)));
-        sbuf[slot][r][h].load(sbase + (srow[r][h] + uint32_t(b >> p.scale_shift) * uint32_t(SV * SSZ)));
+  // Bounded wait that also gives up as soon as another warp has given up.
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int err) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    for (;;) {
+      for (int i = 0; i < 32; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+      if (abort_flag) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        atomicOr(&g_device_status, err);
+        abort_flag = 1;
+        return false;
       }
+    }
   };
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (d < steps) load(d, d);
-  fetch(0);
 
-  // Activation row of this lane in each 8-row tile (clamped: the columns past M
-  // are computed and dropped).
-  uint32_t xrow[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = uint32_t(min(i * 8 + g, p.M - 1) * PITCH + warp * 128 + t * 8);
   float2 acc[RT][MT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[r][i][0] = acc[r][i][1] = make_float2(0.0f, 0.0f);
-  const bool f16 = p.wscale_dtype == TG_DT_F16;
+  const int kw = warp % WK, wr = warp / WK;   // of a computing warp
+  const int g = lane >> 2, t = lane & 3;
 
-  for (int s0 = 0; s0 < steps; s0 += DEPTH) {
+  if (warp == WK * WR) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int slot = 0, filled = 0;
+      uint32_t phase = 0;
+      for (int s = 0; s < steps; ++s) {
+        if (!wait(&empty_bar[slot], phase ^ 1u, DEVERR_PIPE_TIMEOUT)) break;
+        uint8_t* dst = smem4 + uint32_t(slot) * SLOT;
+        mbar_arrive_expect_tx(&full_bar[slot], W_BYTES + uint32_t(p.M) * (WK * 128));
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int s = s0 + d;
-      if (s >= steps) break;
-      if (s % PER == 0) {
-        cp_async_wait_all();
-        __syncthreads();  // this buffer is in, and nobody reads the other one any more
-        if ((s / PER + 1) * KC < p.K) fetch(s / PER + 1);
+        for (int b = 0; b < WK / 2; ++b)
+          tma_load_2d(dst + b * (ROWS * 128), &tma_w, &full_bar[slot], (s * (WK / 2) + b) * 128, n0);
+#pragma unroll
+        for (int b = 0; b < WK; ++b)
+          tma_load_2d(dst + W_BYTES + b * (MT * 1024), &tma_x, &full_bar[slot], (s * WK + b) * 128, 0);
+        ++filled;
+        if (++slot == p.stages) {
+          slot = 0;
+          phase ^= 1u;
+        }
       }
-      if (s * WK + warp < blocks) {
-        const uint8_t* xs = smem4 + ((s / PER) & 1) * buf_bytes + (s % PER) * (WK * 128);
-        uint32_t lo[RT][2][4], hi[RT][2][4];
-        float sc[RT][2][SV];
+      // The loads in flight land before the CTA can exit or reuse the ring (after
+      // a wait gave up too).
+      for (int i = max(0, filled - p.stages); i < filled; ++i)
+        wait(&full_bar[i % p.stages], uint32_t(i / p.stages) & 1u, DEVERR_TMA_TIMEOUT);
+    }
+  } else {
+    stage_scales<ROWS, WK * WR * 32>(p, n0, scale, pitch);
+    named_barrier(1, WK * WR * 32);
+    // ------------------------------------------------------------ products
+    const uint32_t w_off = uint32_t(((kw >> 1) * ROWS + wr * RT * 16 + w_row(g)) * 128 +
+                                    ((((kw & 1) * 4 + t) ^ w_row(g)) << 4));
+    // (Rows from M up hold whatever the slot held: their columns are dropped.)
+    uint32_t x_off[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x_off[j] = W_BYTES + uint32_t(kw * (MT * 1024) + x_row(g) * 128 + (((2 * j + (t >> 1)) ^ x_row(g)) << 4) + (t & 1) * 8);
+    const float* srow = scale + (wr * RT * 16 + w_row(g)) * pitch;
+    const int magic[4] = {__float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC)};
+    const float2 magic2 = make_float2(MAGIC, MAGIC);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int s = 0; s < steps; ++s) {
+      if (!__all_sync(0xffffffffu, wait(&full_bar[slot], phase, DEVERR_TMA_TIMEOUT))) break;
+      const uint8_t* base = smem4 + uint32_t(slot) * SLOT;
+      uint4 w[RT][2];
+      float sc[RT][2][SV];
+      const int si = ((s * WK + kw) >> p.scale_shift) * SV;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[r][h] = *reinterpret_cast<const uint4*>(base + w_off + (r * 16 + h * 8) * 128);
+          const float* q = srow + (r * 16 + h * 8) * pitch + si;
+          if constexpr (SV == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(q);
+            sc[r][h][0] = v.x;
+            sc[r][h][1] = v.y;
+            sc[r][h][2] = v.z;
+            sc[r][h][3] = v.w;
+          } else if constexpr (SV == 2) {
+            const float2 v = *reinterpret_cast<const float2*>(q);
+            sc[r][h][0] = v.x;
+            sc[r][h][1] = v.y;
+          } else {
+            sc[r][h][0] = *q;
+          }
+        }
+      uint32_t lo[RT][2][4], hi[RT][2][4];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t v[4] = {w[r][h].x, w[r][h].y, w[r][h].z, w[r][h].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
+            hi[r][h][j] = v[j] & 0xf0f0f0f0u;
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        uint2 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(base + x_off[j] + i * 1024);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int4 w = wbuf[d][r][h];
-            const uint32_t v[4] = {uint32_t(w.x), uint32_t(w.y), uint32_t(w.z), uint32_t(w.w)};
+          for (int q = 0; q < SV; ++q) {
+            constexpr int MM = 4 / SV;  // products per scale
+            int v[4];
+            mma_s8(v, lo[r][0][q * MM], lo[r][1][q * MM], hi[r][0][q * MM], hi[r][1][q * MM], x[q * MM], magic);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
-              hi[r][h][j] = v[j] & 0xf0f0f0f0u;
-            }
-#pragma unroll
-            for (int i = 0; i < SV; ++i) sc[r][h][i] = sbuf[d][r][h].get(i, f16);
+            for (int j = q * MM + 1; j < q * MM + MM; ++j)
+              mma_s8(v, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[j], v);
+            acc[r][i][0] = fma2(sub2(make_float2(__int_as_float(v[0]), __int_as_float(v[1])), magic2),
+                                make_float2(sc[r][0][q], sc[r][0][q]), acc[r][i][0]);
+            acc[r][i][1] = fma2(sub2(make_float2(__int_as_float(v[2]), __int_as_float(v[3])), magic2),
+                                make_float2(sc[r][1][q], sc[r][1][q]), acc[r][i][1]);
           }
-        if (s + DEPTH < steps) load(d, s + DEPTH);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint2 x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(xs + xrow[i] + j * 32);
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int q = 0; q < SV; ++q) {
-              constexpr int MM = 4 / SV;  // products per scale
-              int v[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = __float_as_int(MAGIC);
-#pragma unroll
-              for (int j = q * MM; j < q * MM + MM; ++j)
-                mma_s8(v, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[j].x, x[j].y);
-              const float2 m2 = make_float2(MAGIC, MAGIC);
-              acc[r][i][0] = fma2(sub2(make_float2(__int_as_float(v[0]), __int_as_float(v[1])), m2),
-                                  make_float2(sc[r][0][q], sc[r][0][q]), acc[r][i][0]);
-              acc[r][i][1] = fma2(sub2(make_float2(__int_as_float(v[2]), __int_as_float(v[3])), m2),
-                                  make_float2(sc[r][1][q], sc[r][1][q]), acc[r][i][1]);
-            }
-        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[slot]);
+      if (++slot == p.stages) {
+        slot = 0;
+        phase ^= 1u;
       }
     }
   }
 
-  // The warps' partial tiles [warp][column][row] into shared memory, added in order.
+  // The warps' partial tiles [warp along K][column][row] over the ring, which
+  // every load has landed in and every warp has left; added in order.
   __syncthreads();
   float* red = reinterpret_cast<float*>(smem4);
+  if (warp < WK * WR) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float* o = red + (warp * COLS + i * 8 + 2 * t) * ROWS + r * 16 + h * 8 + g;
-        o[0] = acc[r][i][h].x;
-        o[ROWS] = acc[r][i][h].y;
-      }
+        for (int h = 0; h < 2; ++h) {
+          float* o = red + (kw * COLS + i * 8) * ROWS + (wr * RT + r) * 16 + h * 8 + w_row(g);
+          o[x_row(2 * t) * ROWS] = acc[r][i][h].x;
+          o[x_row(2 * t + 1) * ROWS] = acc[r][i][h].y;
+        }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < p.M * ROWS; i += THREADS) {
     const int m = i / ROWS, r = i % ROWS;
@@ -293,7 +341,7 @@ __global__ void __launch_bounds__(WK * 32, gemv4::ctas(MT, WK)) gemv_i4_kernel(c
     if (n >= p.N) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WK; ++w) v += red[(w * COLS + m) * ROWS + r];
+    for (int k = 0; k < WK; ++k) v += red[(k * COLS + m) * ROWS + r];
     v = v * 0.0625f * p.xscale[m];
     if (p.bias) v += load_as_f32(p.bias, p.bias_dtype, size_t(n));
     store_f32_as(p.out, p.out_dtype, size_t(m) * p.N + n, v);
