@@ -1096,26 +1096,25 @@ int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, 
 
 // Shared memory of a launch with `stages` ring slots: the ring (or the partial
 // tiles) and the scales.
-uint32_t gemv4_smem(int mt, int rows, int groups, int stages) {
+uint32_t gemv4_smem(int mt, int rows, int groups, bool s4, int stages) {
   using namespace tg::gemv4;
   const uint32_t ring = uint32_t(stages) * (w_bytes(rows) + x_bytes(mt));
-  const uint32_t scales = uint32_t(rows * scale_pitch(groups)) * 4u;
-  return std::max(ring + scales, uint32_t(WK * 8 * mt * rows) * 4u) + 1024u;  // 1024: alignment slack
+  return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) + 1024u;  // 1024: alignment slack
 }
 
 // want: CTAs per SM to make room for; as many ring slots as then fit (two at least).
-template <int MT, int RT, int WR, int SV>
+template <int MT, int RT, int WR, int SV, bool S4>
 int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int want, int dev, cudaStream_t st) {
   using namespace tg::gemv4;
   static uint32_t attr_done[kMaxDevices];
   constexpr uint32_t kStatic = 512;  // barriers and the abort flag, rounded up
-  auto kern = tg::gemv_i4_kernel<MT, RT, WR, SV>;
+  auto kern = tg::gemv_i4_kernel<MT, RT, WR, SV, S4>;
   if (!ensure_smem_attr(kern, dev, kSmemPerCtaMax - kStatic, attr_done)) return TG_ERR_CUDA;
   constexpr int kRows = rows(RT, WR);
   const int steps = (p.K / 128 + WK - 1) / WK;
   int stages = std::min(MAX_STAGES, std::max(2, steps));
   auto fits = [&](int s, int ctas) {
-    return uint64_t(ctas) * (gemv4_smem(MT, kRows, p.groups, s) + kStatic + 1024u) <= kSmemPerSm;
+    return uint64_t(ctas) * (gemv4_smem(MT, kRows, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
   };
   while (want > 1 && !fits(3, want)) --want;
   while (stages > 2 && !fits(stages, want)) --stages;
@@ -1132,7 +1131,7 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(unsigned((int64_t(p.N) + kRows - 1) / kRows));
   cfg.blockDim = dim3(threads(WR));
-  cfg.dynamicSmemBytes = gemv4_smem(MT, kRows, p.groups, stages);
+  cfg.dynamicSmemBytes = gemv4_smem(MT, kRows, p.groups, S4, stages);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1145,10 +1144,14 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
 template <int MT, int RT, int WR>
 int launch_gemv4(const int8_t* xq, const uint8_t* w4, const tg::GemvI4Params& p, int sv, int want, int dev,
                  cudaStream_t st) {
+  const bool s4 = p.wscale_dtype == TG_DT_F32;
   switch (sv) {
-    case 4: return launch_gemv4_t<MT, RT, WR, 4>(xq, w4, p, want, dev, st);
-    case 2: return launch_gemv4_t<MT, RT, WR, 2>(xq, w4, p, want, dev, st);
-    default: return launch_gemv4_t<MT, RT, WR, 1>(xq, w4, p, want, dev, st);
+    case 4: return s4 ? launch_gemv4_t<MT, RT, WR, 4, true>(xq, w4, p, want, dev, st)
+                      : launch_gemv4_t<MT, RT, WR, 4, false>(xq, w4, p, want, dev, st);
+    case 2: return s4 ? launch_gemv4_t<MT, RT, WR, 2, true>(xq, w4, p, want, dev, st)
+                      : launch_gemv4_t<MT, RT, WR, 2, false>(xq, w4, p, want, dev, st);
+    default: return s4 ? launch_gemv4_t<MT, RT, WR, 1, true>(xq, w4, p, want, dev, st)
+                       : launch_gemv4_t<MT, RT, WR, 1, false>(xq, w4, p, want, dev, st);
   }
 }
 

@@ -32,7 +32,7 @@
 //    activation row; lane g's row is picked (w_row, x_row) so that the rows one
 //    shared-memory pass reads lie in different banks.  Blocks past K and rows
 //    past N arrive as zeros, so the loop has no edges.
-//  * The rows' scales are put into shared memory as fp32 at the start.
+//  * The rows' scales, one contiguous stretch, come by one bulk copy at the start.
 //  * The int32 accumulators start at the bits of 1.5 * 2^23, so that the finished
 //    sum v is the fp32 number 1.5 * 2^23 + v (|v| <= 2^21): one paired
 //    subtraction and one paired fma per two outputs and group, no conversion.
@@ -48,10 +48,12 @@ constexpr int MAX_STAGES = 16;
 __host__ __device__ constexpr int threads(int wr) { return 32 * (WK * wr + 1); }
 __host__ __device__ constexpr int rows(int rt, int wr) { return 16 * rt * wr; }
 // Bytes of a ring slot's weights ([two blocks][row][128]) and activations
-// ([block][row][128]); words of a row's scales (eight rows start in different banks).
+// ([block][row][128]), and of the scales of the CTA's rows.
 __host__ __device__ constexpr uint32_t w_bytes(int rows) { return uint32_t(rows) * WK * 64; }
 __host__ __device__ constexpr uint32_t x_bytes(int mt) { return uint32_t(mt) * WK * 1024; }
-__host__ __device__ constexpr int scale_pitch(int groups) { return (groups + 16 + 31) / 32 * 32 + 4; }
+__host__ __device__ constexpr uint32_t scale_bytes(int rows, int groups, bool s4) {
+  return (uint32_t(rows) * uint32_t(groups) * (s4 ? 4u : 2u) + 15u) & ~15u;
+}
 // The weight row and the activation row, of eight, that lanes 4 g .. 4 g + 3 hold.
 // Swizzled, byte chunk c of row r lies at c ^ r: a pass of eight lanes reads 64
 // bytes of w_row 2i and 2i + 1, which differ in bit 2 (other halves of the 128
@@ -91,47 +93,44 @@ __device__ __forceinline__ void store_f32_as(void* out, int dtype, size_t i, flo
   else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(r);
 }
 
-// The scales of rows [n0, n0 + ROWS) to shared memory as fp32, `pitch` words a row,
-// by THREADS threads: one contiguous, 16-byte aligned stretch (n0 is a multiple
-// of 16), read 16 bytes at a time.  Zeros behind a row's last group, for the
-// blocks past K; the rows past N are dropped and left alone.
-template <int ROWS, int THREADS>
-__device__ __forceinline__ void stage_scales(const GemvI4Params& p, int n0, float* scale, int pitch) {
-  const bool f32 = p.wscale_dtype == TG_DT_F32, f16 = p.wscale_dtype == TG_DT_F16;
-  const int per = f32 ? 4 : 8;
-  const int valid = min(ROWS, p.N - n0) * p.groups;
-  const char* src = static_cast<const char*>(p.wscale) + size_t(n0) * size_t(p.groups) * (f32 ? 4 : 2);
-#pragma unroll 4
-  for (int i = threadIdx.x * per; i < valid; i += THREADS * per) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (i + per <= valid) {
-      v = *reinterpret_cast<const uint4*>(src + i * (16 / per));
-    } else {  // the last, part-filled 16 bytes of the tensor
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-      for (int k = 0; i + k < valid; ++k) {
-        if (f32) w[k] = reinterpret_cast<const uint32_t*>(src)[i + k];
-        else w[k >> 1] |= uint32_t(reinterpret_cast<const unsigned short*>(src)[i + k]) << ((k & 1) * 16);
-      }
-      v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    int r = i / p.groups, c = i - r * p.groups;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k < per && i + k < valid) {
-        const uint32_t h = (k & 1) ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
-        scale[r * pitch + c] = f32 ? __uint_as_float(w[k & 3])
-                                   : (f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h)))
-                                          : __uint_as_float(h << 16));
-      }
-      if (++c == p.groups) {
-        c = 0;
-        ++r;
-      }
+// An untiled copy of `bytes` (a multiple of 16) to shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// One block's scales of a row: SV of them, as stored.
+template <int SV, bool S4>
+struct RawScale {
+  uint32_t v[S4 ? SV : (SV + 1) / 2];
+  __device__ __forceinline__ void load(const uint8_t* q) {
+    constexpr int BYTES = SV * (S4 ? 4 : 2);
+    if constexpr (BYTES == 2) {
+      v[0] = *reinterpret_cast<const unsigned short*>(q);
+    } else if constexpr (BYTES == 4) {
+      v[0] = *reinterpret_cast<const uint32_t*>(q);
+    } else if constexpr (BYTES == 8) {
+      const uint2 a = *reinterpret_cast<const uint2*>(q);
+      v[0] = a.x;
+      v[1] = a.y;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(q);
+      v[0] = a.x;
+      v[1] = a.y;
+      v[2] = a.z;
+      v[3] = a.w;
     }
   }
-  for (int i = threadIdx.x; i < ROWS * 16; i += THREADS) scale[(i >> 4) * pitch + p.groups + (i & 15)] = 0.0f;
-}
+  __device__ __forceinline__ float get(int i, bool f16) const {
+    if constexpr (S4) {
+      return __uint_as_float(v[i]);
+    } else {
+      const uint32_t h = (i & 1) ? v[i / 2] >> 16 : v[i / 2] & 0xffffu;
+      return f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16);
+    }
+  }
+};
 
 // d = a (16 x 32, rows) * b (32 x 8, columns) + c, int8 -> int32.
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b,
@@ -144,8 +143,8 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 
 // MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per warp; WR:
 // warps along N; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128
-// and 256: 1).
-template <int MT, int RT, int WR, int SV>
+// and 256: 1); S4: fp32 scales.
+template <int MT, int RT, int WR, int SV, bool S4>
 __global__ void __launch_bounds__(gemv4::threads(WR))
     gemv_i4_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                    const GemvI4Params p) {
@@ -160,14 +159,21 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
   uint8_t* const smem4 = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
   __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t scale_bar;
   __shared__ volatile int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * ROWS;
-  const int steps = (p.K / 128 + WK - 1) / WK;
+  const int blocks = p.K / 128;
+  const int steps = (blocks + WK - 1) / WK;
   constexpr uint32_t SLOT = W_BYTES + x_bytes(MT);
-  const int pitch = scale_pitch(p.groups);
-  float* const scale = reinterpret_cast<float*>(smem4 + uint32_t(p.stages) * SLOT);
+  // The scales of this CTA's rows are one stretch of wscale (16-byte aligned: n0 is
+  // a multiple of 16); its last bytes may not fill 16.
+  constexpr uint32_t SSZ = S4 ? 4 : 2;
+  uint8_t* const scale = smem4 + uint32_t(p.stages) * SLOT;
+  const uint8_t* const scale_src = static_cast<const uint8_t*>(p.wscale) + size_t(n0) * size_t(p.groups) * SSZ;
+  const uint32_t scale_len = uint32_t(min(ROWS, p.N - n0)) * uint32_t(p.groups) * SSZ;
+  const uint32_t scale_bulk = scale_len & ~15u;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tmap(&tma_w);
@@ -176,6 +182,7 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], WK * WR);
     }
+    mbar_init(&scale_bar, 1);
     fence_mbar_init();
     abort_flag = 0;
     // Only into L2: the kernel before may be the one that wrote the weight.
@@ -213,6 +220,8 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
     if (lane == 0) {
       int slot = 0, filled = 0;
       uint32_t phase = 0;
+      mbar_arrive_expect_tx(&scale_bar, scale_bulk);
+      if (scale_bulk) bulk_load(scale, scale_src, scale_bulk, &scale_bar);
       for (int s = 0; s < steps; ++s) {
         if (!wait(&empty_bar[slot], phase ^ 1u, DEVERR_PIPE_TIMEOUT)) break;
         uint8_t* dst = smem4 + uint32_t(slot) * SLOT;
@@ -233,10 +242,14 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
       // a wait gave up too).
       for (int i = max(0, filled - p.stages); i < filled; ++i)
         wait(&full_bar[i % p.stages], uint32_t(i / p.stages) & 1u, DEVERR_TMA_TIMEOUT);
+      wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT);
     }
   } else {
-    stage_scales<ROWS, WK * WR * 32>(p, n0, scale, pitch);
-    named_barrier(1, WK * WR * 32);
+    if (scale_bulk != scale_len) {  // (the same for all warps)
+      if (threadIdx.x < 16 && scale_bulk + threadIdx.x < scale_len)
+        scale[scale_bulk + threadIdx.x] = scale_src[scale_bulk + threadIdx.x];
+      named_barrier(1, WK * WR * 32);
+    }
     // ------------------------------------------------------------ products
     const uint32_t w_off = uint32_t(((kw >> 1) * ROWS + wr * RT * 16 + w_row(g)) * 128 +
                                     ((((kw & 1) * 4 + t) ^ w_row(g)) << 4));
@@ -245,69 +258,66 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       x_off[j] = W_BYTES + uint32_t(kw * (MT * 1024) + x_row(g) * 128 + (((2 * j + (t >> 1)) ^ x_row(g)) << 4) + (t & 1) * 8);
-    const float* srow = scale + (wr * RT * 16 + w_row(g)) * pitch;
+    // (The rows past N read whatever lies behind the scales: they are dropped.)
+    const uint32_t spitch = uint32_t(p.groups) * SSZ;
+    const uint8_t* srow = scale + uint32_t(wr * RT * 16 + w_row(g)) * spitch;
+    const bool f16 = p.wscale_dtype == TG_DT_F16;
     const int magic[4] = {__float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC)};
     const float2 magic2 = make_float2(MAGIC, MAGIC);
     int slot = 0;
     uint32_t phase = 0;
-    for (int s = 0; s < steps; ++s) {
+    const bool go = __all_sync(0xffffffffu, wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT));
+    for (int s = 0; go && s < steps; ++s) {
       if (!__all_sync(0xffffffffu, wait(&full_bar[slot], phase, DEVERR_TMA_TIMEOUT))) break;
-      const uint8_t* base = smem4 + uint32_t(slot) * SLOT;
-      uint4 w[RT][2];
-      float sc[RT][2][SV];
-      const int si = ((s * WK + kw) >> p.scale_shift) * SV;
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          w[r][h] = *reinterpret_cast<const uint4*>(base + w_off + (r * 16 + h * 8) * 128);
-          const float* q = srow + (r * 16 + h * 8) * pitch + si;
-          if constexpr (SV == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(q);
-            sc[r][h][0] = v.x;
-            sc[r][h][1] = v.y;
-            sc[r][h][2] = v.z;
-            sc[r][h][3] = v.w;
-          } else if constexpr (SV == 2) {
-            const float2 v = *reinterpret_cast<const float2*>(q);
-            sc[r][h][0] = v.x;
-            sc[r][h][1] = v.y;
-          } else {
-            sc[r][h][0] = *q;
-          }
-        }
-      uint32_t lo[RT][2][4], hi[RT][2][4];
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t v[4] = {w[r][h].x, w[r][h].y, w[r][h].z, w[r][h].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
-            hi[r][h][j] = v[j] & 0xf0f0f0f0u;
-          }
-        }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        uint2 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(base + x_off[j] + i * 1024);
+      const int b = s * WK + kw;
+      if (b < blocks) {
+        const uint8_t* base = smem4 + uint32_t(slot) * SLOT;
+        uint4 w[RT][2];
+        float sc[RT][2][SV];
+        const uint32_t si = uint32_t(b >> p.scale_shift) * (SV * SSZ);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int q = 0; q < SV; ++q) {
-            constexpr int MM = 4 / SV;  // products per scale
-            int v[4];
-            mma_s8(v, lo[r][0][q * MM], lo[r][1][q * MM], hi[r][0][q * MM], hi[r][1][q * MM], x[q * MM], magic);
+          for (int h = 0; h < 2; ++h) {
+            w[r][h] = *reinterpret_cast<const uint4*>(base + w_off + (r * 16 + h * 8) * 128);
+            RawScale<SV, S4> raw;
+            raw.load(srow + (r * 16 + h * 8) * spitch + si);
 #pragma unroll
-            for (int j = q * MM + 1; j < q * MM + MM; ++j)
-              mma_s8(v, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[j], v);
-            acc[r][i][0] = fma2(sub2(make_float2(__int_as_float(v[0]), __int_as_float(v[1])), magic2),
-                                make_float2(sc[r][0][q], sc[r][0][q]), acc[r][i][0]);
-            acc[r][i][1] = fma2(sub2(make_float2(__int_as_float(v[2]), __int_as_float(v[3])), magic2),
-                                make_float2(sc[r][1][q], sc[r][1][q]), acc[r][i][1]);
+            for (int i = 0; i < SV; ++i) sc[r][h][i] = raw.get(i, f16);
           }
+        uint32_t lo[RT][2][4], hi[RT][2][4];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t v[4] = {w[r][h].x, w[r][h].y, w[r][h].z, w[r][h].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
+              hi[r][h][j] = v[j] & 0xf0f0f0f0u;
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          uint2 x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(base + x_off[j] + i * 1024);
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int q = 0; q < SV; ++q) {
+              constexpr int MM = 4 / SV;  // products per scale
+              int v[4];
+              mma_s8(v, lo[r][0][q * MM], lo[r][1][q * MM], hi[r][0][q * MM], hi[r][1][q * MM], x[q * MM], magic);
+#pragma unroll
+              for (int j = q * MM + 1; j < q * MM + MM; ++j)
+                mma_s8(v, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[j], v);
+              acc[r][i][0] = fma2(sub2(make_float2(__int_as_float(v[0]), __int_as_float(v[1])), magic2),
+                                  make_float2(sc[r][0][q], sc[r][0][q]), acc[r][i][0]);
+              acc[r][i][1] = fma2(sub2(make_float2(__int_as_float(v[2]), __int_as_float(v[3])), magic2),
+                                  make_float2(sc[r][1][q], sc[r][1][q]), acc[r][i][1]);
+            }
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[slot]);
