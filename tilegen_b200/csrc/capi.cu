@@ -1094,12 +1094,29 @@ int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, 
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
+// 3-D tiled tensor map over rows of bytes (a multiple of 128) cut into 128-byte
+// blocks: (byte of the block, row, block), 128-byte swizzle.  What lies behind the
+// last block reads as zero.
+bool make_tmap_blocks(CUtensorMap* m, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows,
+                      uint32_t box_blocks) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {128, rows, row_bytes / 128};
+  cuuint64_t strides[2] = {row_bytes, 128};
+  cuuint32_t box[3] = {128, box_rows, box_blocks};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Shared memory of a launch with `stages` ring slots: the ring (or the partial
 // tiles) and the scales.
-uint32_t gemv4_smem(int mt, int rows, int groups, bool s4, int stages) {
+uint32_t gemv4_smem(int m, int mt, int rows, int groups, bool s4, int stages) {
   using namespace tg::gemv4;
-  const uint32_t ring = uint32_t(stages) * (w_bytes(rows) + x_bytes(mt));
-  return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) + 1024u;  // 1024: alignment slack
+  const uint32_t ring = uint32_t(stages) * (w_bytes(rows) + x_bytes(m));
+  return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) +
+         2048u;  // alignment, and what the reads of rows past m may overrun
 }
 
 // want: CTAs per SM to make room for; as many ring slots as then fit (two at least).
@@ -1114,7 +1131,7 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
   const int steps = (p.K / 128 + WK - 1) / WK;
   int stages = std::min(MAX_STAGES, std::max(2, steps));
   auto fits = [&](int s, int ctas) {
-    return uint64_t(ctas) * (gemv4_smem(MT, kRows, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
+    return uint64_t(ctas) * (gemv4_smem(p.M, MT, kRows, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
   };
   while (want > 1 && !fits(3, want)) --want;
   while (stages > 2 && !fits(stages, want)) --stages;
@@ -1124,14 +1141,13 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
   CUtensorMap tw, tx;
   if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w4, uint64_t(p.K) / 2, uint64_t(p.N), uint64_t(p.K) / 2, 128,
                     uint32_t(kRows), CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, uint64_t(p.K), uint64_t(p.M), uint64_t(p.K), 128,
-                    uint32_t(p.M), CU_TENSOR_MAP_SWIZZLE_128B))
+      !make_tmap_blocks(&tx, xq, uint64_t(p.K), uint64_t(p.M), uint32_t(p.M), WK))
     return TG_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(unsigned((int64_t(p.N) + kRows - 1) / kRows));
   cfg.blockDim = dim3(threads(WR));
-  cfg.dynamicSmemBytes = gemv4_smem(MT, kRows, p.groups, S4, stages);
+  cfg.dynamicSmemBytes = gemv4_smem(p.M, MT, kRows, p.groups, S4, stages);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1193,10 +1209,11 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   // CTAs an SM would get if all ran at once.
   const int64_t tiles = (N + 15) / 16;
   const int want = int(std::max<int64_t>(1, std::min<int64_t>(7, (tiles + info.sms_all - 1) / info.sms_all)));
-  if (M <= 8) return launch_gemv4<1, 1, 1>(xq, w4, p, sv, want, dev, st);
-  if (M <= 16) return launch_gemv4<2, 2, 1>(xq, w4, p, sv, std::min(3, (want + 1) / 2), dev, st);
+  if (M <= 8) return launch_gemv4<1, 2, 1>(xq, w4, p, sv, std::min(4, (want + 1) / 2), dev, st);
+  if (M <= 16) return want > 3 ? launch_gemv4<2, 2, 2>(xq, w4, p, sv, std::min(2, (want + 3) / 4), dev, st)
+                               : launch_gemv4<2, 1, 2>(xq, w4, p, sv, std::min(3, (want + 1) / 2), dev, st);
   if (M <= 32) return launch_gemv4<4, 2, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
-  const int rc = launch_gemv4<8, 2, 2>(xq, w4, p, sv, 1, dev, st);
+  const int rc = launch_gemv4<8, 2, 3>(xq, w4, p, sv, 1, dev, st);
   // Very long rows of fine scales leave no room for 64 rows of them.
   return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1>(xq, w4, p, sv, 1, dev, st) : rc;
 }

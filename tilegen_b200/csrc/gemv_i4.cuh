@@ -28,7 +28,8 @@
 //    row's bits depend neither on M nor on the other rows.
 //  * Both come in boxes of 128 bytes a row with the 128-byte swizzle (narrower
 //    rows, laid out for the reads, made the TMA unit the bound: it takes rows
-//    at a fixed rate).  A quad reads 64 bytes of a weight row and 32 of an
+//    at a fixed rate); a step's activations are one copy, by a
+//    three-dimensional map.  A quad reads 64 bytes of a weight row and 32 of an
 //    activation row; lane g's row is picked (w_row, x_row) so that the rows one
 //    shared-memory pass reads lie in different banks.  Blocks past K and rows
 //    past N arrive as zeros, so the loop has no edges.
@@ -50,7 +51,7 @@ __host__ __device__ constexpr int rows(int rt, int wr) { return 16 * rt * wr; }
 // Bytes of a ring slot's weights ([two blocks][row][128]) and activations
 // ([block][row][128]), and of the scales of the CTA's rows.
 __host__ __device__ constexpr uint32_t w_bytes(int rows) { return uint32_t(rows) * WK * 64; }
-__host__ __device__ constexpr uint32_t x_bytes(int mt) { return uint32_t(mt) * WK * 1024; }
+__host__ __device__ constexpr uint32_t x_bytes(int m) { return (uint32_t(m) * WK * 128 + 1023u) & ~1023u; }
 __host__ __device__ constexpr uint32_t scale_bytes(int rows, int groups, bool s4) {
   return (uint32_t(rows) * uint32_t(groups) * (s4 ? 4u : 2u) + 15u) & ~15u;
 }
@@ -91,6 +92,13 @@ __device__ __forceinline__ void store_f32_as(void* out, int dtype, size_t i, flo
   if (dtype == TG_DT_F32) static_cast<float*>(out)[i] = r;
   else if (dtype == TG_DT_F16) static_cast<__half*>(out)[i] = __float2half_rn(r);
   else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(r);
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
 
 // An untiled copy of `bytes` (a multiple of 16) to shared memory, completing on `bar`.
@@ -166,11 +174,11 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
   const int n0 = blockIdx.x * ROWS;
   const int blocks = p.K / 128;
   const int steps = (blocks + WK - 1) / WK;
-  constexpr uint32_t SLOT = W_BYTES + x_bytes(MT);
+  const uint32_t slot_bytes = W_BYTES + x_bytes(p.M);
   // The scales of this CTA's rows are one stretch of wscale (16-byte aligned: n0 is
   // a multiple of 16); its last bytes may not fill 16.
   constexpr uint32_t SSZ = S4 ? 4 : 2;
-  uint8_t* const scale = smem4 + uint32_t(p.stages) * SLOT;
+  uint8_t* const scale = smem4 + uint32_t(p.stages) * slot_bytes;
   const uint8_t* const scale_src = static_cast<const uint8_t*>(p.wscale) + size_t(n0) * size_t(p.groups) * SSZ;
   const uint32_t scale_len = uint32_t(min(ROWS, p.N - n0)) * uint32_t(p.groups) * SSZ;
   const uint32_t scale_bulk = scale_len & ~15u;
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
     fence_mbar_init();
     abort_flag = 0;
     // Only into L2: the kernel before may be the one that wrote the weight.
-    for (int s = 0; s < 2 * p.prefetch; ++s) tma_prefetch_l2_2d(&tma_w, s * 128, n0);
+    for (int s = 0; s < (WK / 2) * p.prefetch; ++s) tma_prefetch_l2_2d(&tma_w, s * 128, n0);
   }
   __syncthreads();
   pdl_wait();
@@ -224,14 +232,12 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
       if (scale_bulk) bulk_load(scale, scale_src, scale_bulk, &scale_bar);
       for (int s = 0; s < steps; ++s) {
         if (!wait(&empty_bar[slot], phase ^ 1u, DEVERR_PIPE_TIMEOUT)) break;
-        uint8_t* dst = smem4 + uint32_t(slot) * SLOT;
+        uint8_t* dst = smem4 + uint32_t(slot) * slot_bytes;
         mbar_arrive_expect_tx(&full_bar[slot], W_BYTES + uint32_t(p.M) * (WK * 128));
 #pragma unroll
         for (int b = 0; b < WK / 2; ++b)
           tma_load_2d(dst + b * (ROWS * 128), &tma_w, &full_bar[slot], (s * (WK / 2) + b) * 128, n0);
-#pragma unroll
-        for (int b = 0; b < WK; ++b)
-          tma_load_2d(dst + W_BYTES + b * (MT * 1024), &tma_x, &full_bar[slot], (s * WK + b) * 128, 0);
+        tma_load_3d(dst + W_BYTES, &tma_x, &full_bar[slot], 0, 0, s * WK);
         ++filled;
         if (++slot == p.stages) {
           slot = 0;
@@ -253,11 +259,13 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
     // ------------------------------------------------------------ products
     const uint32_t w_off = uint32_t(((kw >> 1) * ROWS + wr * RT * 16 + w_row(g)) * 128 +
                                     ((((kw & 1) * 4 + t) ^ w_row(g)) << 4));
-    // (Rows from M up hold whatever the slot held: their columns are dropped.)
+    // (Rows from M up are whatever lies behind: their columns are dropped.)  A row's
+    // swizzle follows from its place in the slot.
+    const int xr = kw * p.M + x_row(g);
     uint32_t x_off[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      x_off[j] = W_BYTES + uint32_t(kw * (MT * 1024) + x_row(g) * 128 + (((2 * j + (t >> 1)) ^ x_row(g)) << 4) + (t & 1) * 8);
+      x_off[j] = W_BYTES + uint32_t(xr * 128 + (((2 * j + (t >> 1)) ^ (xr & 7)) << 4) + (t & 1) * 8);
     // (The rows past N read whatever lies behind the scales: they are dropped.)
     const uint32_t spitch = uint32_t(p.groups) * SSZ;
     const uint8_t* srow = scale + uint32_t(wr * RT * 16 + w_row(g)) * spitch;
@@ -271,7 +279,7 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
       if (!__all_sync(0xffffffffu, wait(&full_bar[slot], phase, DEVERR_TMA_TIMEOUT))) break;
       const int b = s * WK + kw;
       if (b < blocks) {
-        const uint8_t* base = smem4 + uint32_t(slot) * SLOT;
+        const uint8_t* base = smem4 + uint32_t(slot) * slot_bytes;
         uint4 w[RT][2];
         float sc[RT][2][SV];
         const uint32_t si = uint32_t(b >> p.scale_shift) * (SV * SSZ);
