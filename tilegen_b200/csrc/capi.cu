@@ -1213,9 +1213,13 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (M <= 16) return want > 3 ? launch_gemv4<2, 2, 2>(xq, w4, p, sv, std::min(2, (want + 3) / 4), dev, st)
                                : launch_gemv4<2, 1, 2>(xq, w4, p, sv, std::min(3, (want + 1) / 2), dev, st);
   if (M <= 32) return launch_gemv4<4, 2, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
-  const int rc = launch_gemv4<8, 2, 3>(xq, w4, p, sv, 1, dev, st);
-  // Very long rows of fine scales leave no room for 64 rows of them.
-  return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1>(xq, w4, p, sv, 1, dev, st) : rc;
+  // 64 or 96 rows a CTA, one CTA per SM: whichever takes the fewer rows of them in all.
+  const int64_t t32 = (N + 31) / 32, sms = info.sms_all;
+  const int64_t cost2 = (t32 + 2 * sms - 1) / (2 * sms) * 2, cost3 = (t32 + 3 * sms - 1) / (3 * sms) * 3;
+  const int rc = cost3 < cost2 ? launch_gemv4<8, 2, 3>(xq, w4, p, sv, 1, dev, st)
+                               : launch_gemv4<8, 2, 2>(xq, w4, p, sv, 1, dev, st);
+  // Very long rows of fine scales leave no room for so many rows of them.
+  return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1>(xq, w4, p, sv, 2, dev, st) : rc;
 }
 
 }  // extern "C"

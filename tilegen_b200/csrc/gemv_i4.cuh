@@ -37,6 +37,8 @@
 //  * The int32 accumulators start at the bits of 1.5 * 2^23, so that the finished
 //    sum v is the fp32 number 1.5 * 2^23 + v (|v| <= 2^21): one paired
 //    subtraction and one paired fma per two outputs and group, no conversion.
+//    With 64 columns and several groups a block the conversions, on another
+//    pipe than the fmas, are the faster way (61 rows, groups of 32: 29 us, not 39).
 #pragma once
 
 #include "common.cuh"
@@ -143,7 +145,7 @@ struct RawScale {
 // d = a (16 x 32, rows) * b (32 x 8, columns) + c, int8 -> int32.
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b,
                                        const int (&c)[4]) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
@@ -153,7 +155,7 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 // warps along N; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128
 // and 256: 1); S4: fp32 scales.
 template <int MT, int RT, int WR, int SV, bool S4>
-__global__ void __launch_bounds__(gemv4::threads(WR))
+__global__ void __launch_bounds__(gemv4::threads(WR), 1)
     gemv_i4_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                    const GemvI4Params p) {
   using namespace gemv4;
@@ -161,6 +163,7 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
   constexpr int ROWS = rows(RT, WR), COLS = MT * 8;
   constexpr uint32_t W_BYTES = w_bytes(ROWS);
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
+  constexpr bool CONVERT = MT == 8 && SV >= 2;
   // Ring slots [weights | activations], then the scales; the partial tiles of the
   // end lie over the ring.
   extern __shared__ uint8_t smem_raw[];
@@ -270,8 +273,12 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
     const uint32_t spitch = uint32_t(p.groups) * SSZ;
     const uint8_t* srow = scale + uint32_t(wr * RT * 16 + w_row(g)) * spitch;
     const bool f16 = p.wscale_dtype == TG_DT_F16;
-    const int magic[4] = {__float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC), __float_as_int(MAGIC)};
-    const float2 magic2 = make_float2(MAGIC, MAGIC);
+    const int start = CONVERT ? 0 : __float_as_int(MAGIC);
+    const int magic[4] = {start, start, start, start};
+    auto sums = [](int a, int b) {  // two finished accumulators as fp32
+      return CONVERT ? make_float2(__int2float_rn(a), __int2float_rn(b))
+                     : sub2(make_float2(__int_as_float(a), __int_as_float(b)), make_float2(MAGIC, MAGIC));
+    };
     int slot = 0;
     uint32_t phase = 0;
     const bool go = __all_sync(0xffffffffu, wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT));
@@ -305,26 +312,39 @@ __global__ void __launch_bounds__(gemv4::threads(WR))
               hi[r][h][j] = v[j] & 0xf0f0f0f0u;
             }
           }
+        // IB column tiles at a time, all their products first: a product's result
+        // takes about 35 cycles, so neighbouring ones must not wait for each other.
+        constexpr int IB = MT >= 2 && SV <= 2 ? 2 : 1;
+        constexpr int MM = 4 / SV;  // products per scale
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint2 x[4];
+        for (int i0 = 0; i0 < MT; i0 += IB) {
+          uint2 x[IB][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(base + x_off[j] + i * 1024);
+          for (int i = 0; i < IB; ++i)
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
+            for (int j = 0; j < 4; ++j) x[i][j] = *reinterpret_cast<const uint2*>(base + x_off[j] + (i0 + i) * 1024);
+          int v[IB][RT][SV][4];
 #pragma unroll
-            for (int q = 0; q < SV; ++q) {
-              constexpr int MM = 4 / SV;  // products per scale
-              int v[4];
-              mma_s8(v, lo[r][0][q * MM], lo[r][1][q * MM], hi[r][0][q * MM], hi[r][1][q * MM], x[q * MM], magic);
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int j = q * MM + 1; j < q * MM + MM; ++j)
-                mma_s8(v, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[j], v);
-              acc[r][i][0] = fma2(sub2(make_float2(__int_as_float(v[0]), __int_as_float(v[1])), magic2),
-                                  make_float2(sc[r][0][q], sc[r][0][q]), acc[r][i][0]);
-              acc[r][i][1] = fma2(sub2(make_float2(__int_as_float(v[2]), __int_as_float(v[3])), magic2),
-                                  make_float2(sc[r][1][q], sc[r][1][q]), acc[r][i][1]);
-            }
+            for (int i = 0; i < IB; ++i)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                int(&d)[4] = v[i][r][j / MM];
+                if (j % MM == 0) mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], magic);
+                else mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], d);
+              }
+#pragma unroll
+          for (int q = 0; q < SV; ++q)
+#pragma unroll
+            for (int i = 0; i < IB; ++i)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                const int(&d)[4] = v[i][r][q];
+                float2(&o)[2] = acc[r][i0 + i];
+                o[0] = fma2(sums(d[0], d[1]), make_float2(sc[r][0][q], sc[r][0][q]), o[0]);
+                o[1] = fma2(sums(d[2], d[3]), make_float2(sc[r][1][q], sc[r][1][q]), o[1]);
+              }
         }
       }
       __syncwarp();
