@@ -134,6 +134,21 @@ def test_route_no_tokens_strides_and_refusals(cuda):
             ops.route_experts(*args)
 
 
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("e,top_k,dtype", [(1, 1, torch.float32), (2, 2, torch.float16), (31, 2, torch.float32), (32, 1, torch.bfloat16), (33, 4, torch.float32),
+                                           (64, 3, torch.bfloat16), (128, 8, torch.float16)])
+def test_route_many_tokens_few_experts(cuda, e, top_k, dtype, renormalize):
+    """From 16384 tokens a thread takes a token: ties, closed experts, padded tokens, NaN, the last warp part-filled."""
+    t = 16384 + 45
+    x = (torch.randn(t, e, generator=_gen(e), device=cuda) * 4).round().mul(0.5).to(dtype)  # many equal logits
+    x[::11] = -math.inf
+    x[1::13, e // 2] = -math.inf
+    x[5, 0] = math.nan
+    x[6, e - 1] = math.inf
+    x[t - 1] = 0
+    _check_route(x, top_k, renormalize)
+
+
 def test_route_many_tokens(cuda):
     """65521 tokens against torch's own sorts (integers only)."""
     t, e, top_k = 65521, 160, 6

@@ -1235,14 +1235,28 @@ int route_per_block(int64_t T) {
   return int(per);
 }
 
+template <int K>
+int launch_route_rows(const tg::RouteParams& p, int dev, cudaStream_t st) {
+  using namespace tg::route;
+  static uint32_t attr_done[kMaxDevices];
+  auto kern = tg::route_rows_kernel<K>;
+  if (!ensure_smem_attr(kern, dev, uint32_t(ROW_THREADS * (ROW_MAX_E | 1) * 4), attr_done)) return TG_ERR_CUDA;
+  return launch_dependent(kern, p, dim3(unsigned(p.blocks)), ROW_THREADS, uint32_t(ROW_THREADS * (p.E | 1) * 4), st);
+}
+
 template <int EPL>
-int launch_route(const tg::RouteParams& p, cudaStream_t st) {
+int launch_route(const tg::RouteParams& p, int dev, cudaStream_t st) {
+  using namespace tg::route;
   const dim3 grid{unsigned(p.blocks)};
-  if (p.T <= tg::route::SINGLE)
-    return launch_dependent(tg::route_topk_kernel<EPL, false>, p, grid, tg::route::threads(EPL), 0, st);
-  const int rc = launch_dependent(tg::route_topk_kernel<EPL, true>, p, grid, tg::route::threads(EPL), 0, st);
+  if (p.T <= SINGLE) return launch_dependent(tg::route_topk_kernel<EPL, false>, p, grid, threads(EPL), 0, st);
+  // A thread per token where there are tokens for every SM and a row is short.
+  const bool rows = p.T >= ROW_MIN_T && p.E <= ROW_MAX_E && p.top_k <= ROW_MAX_K;
+  const int rc = !rows ? launch_dependent(tg::route_topk_kernel<EPL, true>, p, grid, threads(EPL), 0, st)
+                 : p.top_k <= 2 ? launch_route_rows<2>(p, dev, st)
+                 : p.top_k <= 4 ? launch_route_rows<4>(p, dev, st)
+                                : launch_route_rows<8>(p, dev, st);
   if (rc != TG_OK) return rc;
-  return launch_dependent(tg::route_place_kernel, p, grid, tg::route::THREADS, 0, st);
+  return launch_dependent(tg::route_place_kernel, p, grid, THREADS, 0, st);
 }
 
 template <int DT>
@@ -1299,12 +1313,15 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
   p.rows = rows;
   p.place = place;
   p.counts = static_cast<int32_t*>(workspace);
-  if (E <= 32) return launch_route<1>(p, st);
-  if (E <= 64) return launch_route<2>(p, st);
-  if (E <= 128) return launch_route<4>(p, st);
-  if (E <= 256) return launch_route<8>(p, st);
-  if (E <= 512) return launch_route<16>(p, st);
-  return launch_route<32>(p, st);
+  int dev;
+  DeviceInfo info;
+  if (!current_device(&dev, &info)) return TG_ERR_CUDA;
+  if (E <= 32) return launch_route<1>(p, dev, st);
+  if (E <= 64) return launch_route<2>(p, dev, st);
+  if (E <= 128) return launch_route<4>(p, dev, st);
+  if (E <= 256) return launch_route<8>(p, dev, st);
+  if (E <= 512) return launch_route<16>(p, dev, st);
+  return launch_route<32>(p, dev, st);
 }
 
 int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place, const float* weights, int64_t T,
