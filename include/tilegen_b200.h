@@ -284,12 +284,20 @@ size_t tg_route_experts_workspace(int64_t T, int64_t E);
  *   offsets  [E + 1] ascending, on the device; read as min(max(., 0), R)
  *   out      [R, N] of out_dtype; N*sizeof(out) % 16 == 0; rows that no group
  *            covers are left as they were
+ *   workspace  tg_int8_grouped_gemm_dequant_workspace(R, E, N, K) bytes, 16-B
+ *            aligned, or NULL: with `rows` and large products the rows are
+ *            gathered there first; without it (or with less) in the kernel.  It
+ *            needs no initial value; calls that share it must not overlap
  * xq, wq and out 16-B aligned; E <= TG_MAX_EXPERTS.  R == 0 is a no-op.
  */
 int tg_int8_grouped_gemm_dequant(const int8_t *xq, const float *xscale, int64_t M, const int8_t *wq,
                                  const float *wscale, int64_t wscale_numel, const void *bias, int bias_dtype,
                                  const int32_t *rows, const int32_t *offsets, int64_t R, int64_t E, int64_t N,
-                                 int64_t K, int out_dtype, void *out, void *stream);
+                                 int64_t K, int out_dtype, void *out, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/* Workspace bytes tg_int8_grouped_gemm_dequant makes use of when `rows` is given (0: none). */
+size_t tg_int8_grouped_gemm_dequant_workspace(int64_t R, int64_t E, int64_t N, int64_t K);
 
 /*
  * Each token's experts' rows added up:

@@ -268,6 +268,23 @@ def test_grouped_bad_indices_are_zero_rows(cuda):
         assert torch.equal(ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, bias, wild, torch.float32, rows=rows), y)
 
 
+def test_grouped_rows_gathered_first(cuda):
+    """Products large enough that the rows are gathered by a pass of their own, bad row numbers among them."""
+    counts, n, k, m = [2600, 0, 1500, 4000], 4096, 4096, 3000
+    assert _lib.lib().tg_int8_grouped_gemm_dequant_workspace(sum(counts), 4, n, k) > 0
+    case = _group_case(counts, n, k, m, torch.bfloat16, seed=4)
+    xq, xs, wq, ws, bias, offsets, rows = case
+    _check_group(case, torch.float16)
+    rows[3], rows[2600], rows[-1] = -1, m, -2 ** 31
+    y = ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, bias, offsets, torch.float32, rows=rows)
+    for r, e in ((3, 0), (2600, 2), (sum(counts) - 1, 3)):
+        assert torch.equal(y[r], bias[e].float())
+    live = torch.ones_like(rows, dtype=torch.bool)
+    live[[3, 2600, -1]] = False
+    rows[~live] = 0
+    assert torch.equal(y[live], _group_ref(xq, xs, wq, ws, bias, offsets, rows, torch.float32)[live])
+
+
 @pytest.mark.parametrize("m", [1, 9, 700])
 def test_grouped_equals_the_single_linear(cuda, m):
     xq, xs, wq, ws, bias, offsets, _ = _group_case([m], 512, 1024, None, torch.float16, seed=m)

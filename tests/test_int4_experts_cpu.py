@@ -163,7 +163,7 @@ def test_route_entry_checks(kwargs, status):
 
 def _grouped(xq=P, xs=P, m=4, wq=P, ws=P, wn=1, bias=None, bdt=0, rows=P, offsets=P, r=8, e=2, n=64, k=64, odt=1, out=P):
     return _lib.lib().tg_int8_grouped_gemm_dequant(xq, xs, m, wq, ws, wn, bias, bdt, rows, offsets, r, e, n, k, odt, out,
-                                                   None)
+                                                   None, 0, None)
 
 
 @pytest.mark.parametrize("kwargs,status", [
@@ -175,6 +175,9 @@ def _grouped(xq=P, xs=P, m=4, wq=P, ws=P, wn=1, bias=None, bdt=0, rows=P, offset
     ({"r": 0, "out": None}, OK), ({"m": 0, "r": 0, "xq": None}, OK),
 ])
 def test_grouped_entry_checks(kwargs, status):
+    need = _lib.lib().tg_int8_grouped_gemm_dequant_workspace
+    assert need(8, 2, 64, 64) == 0 and need(4096, 8, 1024, 1024) == 0
+    assert need(8192, 8, 13824, 5120) == 8192 * 5124
     assert _grouped(**kwargs) == status
 
 

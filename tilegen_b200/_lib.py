@@ -131,7 +131,10 @@ def lib() -> ctypes.CDLL:
         L.tg_route_experts.restype = i32
         L.tg_route_experts_workspace.argtypes = [i64, i64]
         L.tg_route_experts_workspace.restype = ctypes.c_size_t
-        L.tg_int8_grouped_gemm_dequant.argtypes = [p, p, i64, p, p, i64, p, i32, p, p, i64, i64, i64, i64, i32, p, p]
+        L.tg_int8_grouped_gemm_dequant.argtypes = [p, p, i64, p, p, i64, p, i32, p, p, i64, i64, i64, i64, i32, p, p,
+                                                   ctypes.c_size_t, p]
+        L.tg_int8_grouped_gemm_dequant_workspace.argtypes = [i64, i64, i64, i64]
+        L.tg_int8_grouped_gemm_dequant_workspace.restype = ctypes.c_size_t
         L.tg_int8_grouped_gemm_dequant.restype = i32
         L.tg_combine_experts.argtypes = [p, i32, i64, p, p, i64, i32, p, i64, p, p]
         L.tg_combine_experts.restype = i32

@@ -1112,28 +1112,28 @@ bool make_tmap_blocks(CUtensorMap* m, const void* base, uint64_t row_bytes, uint
 
 // Shared memory of a launch with `stages` ring slots: the ring (or the partial
 // tiles) and the scales.
-uint32_t gemv4_smem(int m, int mt, int rows, int groups, bool s4, int stages) {
+uint32_t gemv4_smem(int m, int mt, int rows, int kb, int groups, bool s4, int stages) {
   using namespace tg::gemv4;
-  const uint32_t ring = uint32_t(stages) * (w_bytes(rows) + x_bytes(m));
+  const uint32_t ring = uint32_t(stages) * (w_bytes(kb, rows) + x_bytes(kb, m));
   return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) +
          2048u;  // alignment, and what the reads of rows past m may overrun
 }
 
 // want: CTAs per SM to make room for; as many ring slots as then fit (two at least).
-template <int MT, int RT, int WR, int SV, bool S4>
+template <int MT, int RT, int WR, int KB, int SV, bool S4>
 int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int want, int dev, cudaStream_t st) {
   using namespace tg::gemv4;
   static uint32_t attr_done[kMaxDevices];
   constexpr uint32_t kStatic = 512;  // barriers and the abort flag, rounded up
-  auto kern = tg::gemv_i4_kernel<MT, RT, WR, SV, S4>;
+  auto kern = tg::gemv_i4_kernel<MT, RT, WR, KB, SV, S4>;
   if (!ensure_smem_attr(kern, dev, kSmemPerCtaMax - kStatic, attr_done)) return TG_ERR_CUDA;
   constexpr int kRows = rows(RT, WR);
-  const int steps = (p.K / 128 + WK - 1) / WK;
+  const int steps = (p.K / 128 + KB * WK - 1) / (KB * WK);
   int stages = std::min(MAX_STAGES, std::max(2, steps));
   auto fits = [&](int s, int ctas) {
-    return uint64_t(ctas) * (gemv4_smem(p.M, MT, kRows, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
+    return uint64_t(ctas) * (gemv4_smem(p.M, MT, kRows, KB, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
   };
-  while (want > 1 && !fits(3, want)) --want;
+  while (want > 1 && !fits(std::min(3, stages), want)) --want;
   while (stages > 2 && !fits(stages, want)) --stages;
   if (!fits(stages, 1)) return TG_ERR_UNSUPPORTED;
   p.stages = stages;
@@ -1141,13 +1141,13 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
   CUtensorMap tw, tx;
   if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w4, uint64_t(p.K) / 2, uint64_t(p.N), uint64_t(p.K) / 2, 128,
                     uint32_t(kRows), CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_blocks(&tx, xq, uint64_t(p.K), uint64_t(p.M), uint32_t(p.M), WK))
+      !make_tmap_blocks(&tx, xq, uint64_t(p.K), uint64_t(p.M), uint32_t(p.M), uint32_t(KB * WK)))
     return TG_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(unsigned((int64_t(p.N) + kRows - 1) / kRows));
   cfg.blockDim = dim3(threads(WR));
-  cfg.dynamicSmemBytes = gemv4_smem(p.M, MT, kRows, p.groups, S4, stages);
+  cfg.dynamicSmemBytes = gemv4_smem(p.M, MT, kRows, KB, p.groups, S4, stages);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1157,17 +1157,17 @@ int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int 
   return cudaGetLastError() == cudaSuccess ? TG_OK : TG_ERR_CUDA;
 }
 
-template <int MT, int RT, int WR>
+template <int MT, int RT, int WR, int KB>
 int launch_gemv4(const int8_t* xq, const uint8_t* w4, const tg::GemvI4Params& p, int sv, int want, int dev,
                  cudaStream_t st) {
   const bool s4 = p.wscale_dtype == TG_DT_F32;
   switch (sv) {
-    case 4: return s4 ? launch_gemv4_t<MT, RT, WR, 4, true>(xq, w4, p, want, dev, st)
-                      : launch_gemv4_t<MT, RT, WR, 4, false>(xq, w4, p, want, dev, st);
-    case 2: return s4 ? launch_gemv4_t<MT, RT, WR, 2, true>(xq, w4, p, want, dev, st)
-                      : launch_gemv4_t<MT, RT, WR, 2, false>(xq, w4, p, want, dev, st);
-    default: return s4 ? launch_gemv4_t<MT, RT, WR, 1, true>(xq, w4, p, want, dev, st)
-                       : launch_gemv4_t<MT, RT, WR, 1, false>(xq, w4, p, want, dev, st);
+    case 4: return s4 ? launch_gemv4_t<MT, RT, WR, KB, 4, true>(xq, w4, p, want, dev, st)
+                      : launch_gemv4_t<MT, RT, WR, KB, 4, false>(xq, w4, p, want, dev, st);
+    case 2: return s4 ? launch_gemv4_t<MT, RT, WR, KB, 2, true>(xq, w4, p, want, dev, st)
+                      : launch_gemv4_t<MT, RT, WR, KB, 2, false>(xq, w4, p, want, dev, st);
+    default: return s4 ? launch_gemv4_t<MT, RT, WR, KB, 1, true>(xq, w4, p, want, dev, st)
+                       : launch_gemv4_t<MT, RT, WR, KB, 1, false>(xq, w4, p, want, dev, st);
   }
 }
 
@@ -1206,20 +1206,26 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sv = group == 32 ? 4 : (group == 64 ? 2 : 1);
-  // CTAs an SM would get if all ran at once.
-  const int64_t tiles = (N + 15) / 16;
-  const int want = int(std::max<int64_t>(1, std::min<int64_t>(7, (tiles + info.sms_all - 1) / info.sms_all)));
-  if (M <= 8) return launch_gemv4<1, 2, 1>(xq, w4, p, sv, std::min(4, (want + 1) / 2), dev, st);
-  if (M <= 16) return want > 3 ? launch_gemv4<2, 2, 2>(xq, w4, p, sv, std::min(2, (want + 3) / 4), dev, st)
-                               : launch_gemv4<2, 1, 2>(xq, w4, p, sv, std::min(3, (want + 1) / 2), dev, st);
-  if (M <= 32) return launch_gemv4<4, 2, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
+  // 16-row tiles an SM gets.  Where they are few, a CTA's steps are what takes the
+  // time, and two blocks a step halve them; where they are many, one block a step
+  // leaves room for the rings of more CTAs.  Measured (two blocks / one, us): one
+  // row, 5120 x 5120 5.9 / 6.8, 5120 x 13824 13.6 / 14.7; 15360 x 5120 with 8 rows
+  // 14.0 / 9.6, with 16 rows 17.5 / 11.9.
+  const int64_t tiles = (N + 15) / 16, sms = info.sms_all;
+  const int want = int(std::max<int64_t>(1, std::min<int64_t>(8, (tiles + sms - 1) / sms)));
+  const bool few = want <= 3;
+  if (M <= 8) return few ? launch_gemv4<1, 2, 1, 2>(xq, w4, p, sv, (want + 1) / 2, dev, st)
+                         : launch_gemv4<1, 2, 1, 1>(xq, w4, p, sv, (want + 1) / 2, dev, st);
+  if (M <= 16) return few ? launch_gemv4<2, 1, 2, 2>(xq, w4, p, sv, (want + 1) / 2, dev, st)
+                          : launch_gemv4<2, 2, 2, 1>(xq, w4, p, sv, 2, dev, st);
+  if (M <= 32) return launch_gemv4<4, 2, 1, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
   // 64 or 96 rows a CTA, one CTA per SM: whichever takes the fewer rows of them in all.
-  const int64_t t32 = (N + 31) / 32, sms = info.sms_all;
+  const int64_t t32 = (N + 31) / 32;
   const int64_t cost2 = (t32 + 2 * sms - 1) / (2 * sms) * 2, cost3 = (t32 + 3 * sms - 1) / (3 * sms) * 3;
-  const int rc = cost3 < cost2 ? launch_gemv4<8, 2, 3>(xq, w4, p, sv, 1, dev, st)
-                               : launch_gemv4<8, 2, 2>(xq, w4, p, sv, 1, dev, st);
+  const int rc = cost3 < cost2 ? launch_gemv4<8, 2, 3, 1>(xq, w4, p, sv, 1, dev, st)
+                               : launch_gemv4<8, 2, 2, 1>(xq, w4, p, sv, 1, dev, st);
   // Very long rows of fine scales leave no room for so many rows of them.
-  return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1>(xq, w4, p, sv, 2, dev, st) : rc;
+  return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1, 1>(xq, w4, p, sv, 2, dev, st) : rc;
 }
 
 }  // extern "C"
@@ -1357,6 +1363,18 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
 
 namespace {
 
+// A pass of its own gathers the rows where an expert has 256 of them or more and
+// the products are 1.25e11 multiply-adds or more, about 100 us: measured (in the
+// kernel / in a pass, us) 455 / 420 at 8192 x 13824 x 5120 over 8 experts, 295 / 284
+// and 178 / 171 at 32768 and 16384 x 4096 x 2048 over 64; below, the pass costs
+// what it saves: 63 / 65 at 2048 x 5120 x 5120 over 8, 17.6 / 18.9 at 4096 x 1024 x
+// 1024 over 8, 124 / 123 at 128 rows an expert.
+constexpr int64_t kGatherPassMinRows = 256;
+constexpr double kGatherPassMinWork = 1.25e11;
+
+// Rows an expert has on average, if every expert has some.
+int64_t grouped_avg(int64_t R, int64_t E) { return R / std::max<int64_t>(1, std::min(E, R)); }
+
 // The output's tensor map has to match the kernel's chunk (32 rows x 32 channels).
 template <int TN, int OUT, bool GATHER>
 int launch_grouped_t(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& to, tg::GroupedParams p, int dev,
@@ -1413,10 +1431,18 @@ int launch_grouped_tn(const int8_t* xq, const CUtensorMap& tw, const CUtensorMap
 
 extern "C" {
 
+size_t tg_int8_grouped_gemm_dequant_workspace(int64_t R, int64_t E, int64_t N, int64_t K) {
+  if (R <= 0 || E <= 0 || N <= 0 || K <= 0 || grouped_avg(R, E) < kGatherPassMinRows ||
+      double(R) * double(N) * double(K) < kGatherPassMinWork)
+    return 0;
+  return size_t(R) * size_t(K + 4);
+}
+
 int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t M, const int8_t* wq,
                                  const float* wscale, int64_t wscale_numel, const void* bias, int bias_dtype,
                                  const int32_t* rows, const int32_t* offsets, int64_t R, int64_t E, int64_t N,
-                                 int64_t K, int out_dtype, void* out, void* stream) {
+                                 int64_t K, int out_dtype, void* out, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
   if (M < 0 || R < 0 || E <= 0 || N <= 0 || K <= 0) return TG_ERR_INVALID_ARG;
   if (!is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
   if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
@@ -1434,6 +1460,26 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   int dev;
   DeviceInfo info;
   if (!current_device(&dev, &info)) return TG_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t need = rows ? tg_int8_grouped_gemm_dequant_workspace(R, E, N, K) : 0;
+  if (need > 0 && workspace && workspace_bytes >= need) {
+    if (!aligned16(workspace)) return TG_ERR_MISALIGNED;
+    tg::GatherRowsParams g;
+    g.xq = xq;
+    g.xscale = xscale;
+    g.rows = rows;
+    g.q = static_cast<int8_t*>(workspace);
+    g.scale = reinterpret_cast<float*>(g.q + R * K);
+    g.M = int(M);
+    g.R = int(R);
+    g.K = int(K);
+    const int rc = launch_dependent(tg::gather_rows_kernel, g, dim3(unsigned((R + 7) / 8)), 256, 0, st);
+    if (rc != TG_OK) return rc;
+    xq = g.q;
+    xscale = g.scale;
+    rows = nullptr;
+    M = R;
+  }
   using namespace tg::grouped;
   CUtensorMap tw, to;
   if (!make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, uint64_t(K), uint64_t(E * N), uint64_t(K), BK, BNW,
@@ -1459,9 +1505,7 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   p.N = int(N);
   p.K = int(K);
   p.out = out;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Rows an expert has on average, if every expert has some.
-  const int64_t avg = R / std::min<int64_t>(E, R);
+  const int64_t avg = grouped_avg(R, E);
   if (avg <= 24) return launch_grouped_tn<64>(xq, tw, to, p, out_dtype, dev, info.sms, st);
   if (avg <= 64) return launch_grouped_tn<128>(xq, tw, to, p, out_dtype, dev, info.sms, st);
   return launch_grouped_tn<256>(xq, tw, to, p, out_dtype, dev, info.sms, st);

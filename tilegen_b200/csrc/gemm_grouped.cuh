@@ -430,4 +430,32 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
   }
 }
 
+// The gather as a pass of its own, for groups large enough that the tensor cores
+// are the bound: the TMA unit takes gathered rows at a quarter of the rate of
+// whole boxes, and a tile's rows would be gathered again for every 256 output
+// channels.  A warp copies a row (and its scale); a row number outside xq gives
+// zeros.
+struct GatherRowsParams {
+  const int8_t* xq;      // [M, K]
+  const float* xscale;   // [M]
+  const int32_t* rows;   // [R]
+  int8_t* q;             // [R, K] out
+  float* scale;          // [R] out
+  int M, R, K;
+};
+
+__global__ void __launch_bounds__(256) gather_rows_kernel(const GatherRowsParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= p.R) return;
+  const int a = p.rows[r];
+  const bool ok = a >= 0 && a < p.M;
+  const int4* src = reinterpret_cast<const int4*>(p.xq + size_t(ok ? a : 0) * p.K);
+  int4* dst = reinterpret_cast<int4*>(p.q + size_t(r) * p.K);
+  if (lane == 0) p.scale[r] = ok ? p.xscale[a] : 0.0f;
+#pragma unroll 4
+  for (int i = lane; i < p.K / 16; i += 32) dst[i] = ok ? src[i] : make_int4(0, 0, 0, 0);
+}
+
 }  // namespace tg

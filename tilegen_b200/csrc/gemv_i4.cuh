@@ -22,9 +22,9 @@
 // the products are 20 % of its measured 1140 TOP/s at the weight's HBM rate, and
 // tcgen05 would need the unpacked weight written back to shared memory); the
 // activations are the N operand, 8 rows a product.
-//  * A CTA has WR * RT * 16 weight rows and all of K.  A step is four blocks of 128
-//    codes, one for each of the four warps along K, so the activations of a step
-//    are read once per CTA.  The order of all additions depends on K alone: a
+//  * A CTA has WR * RT * 16 weight rows and all of K.  A step is one or two blocks
+//    of 128 codes for each of the four warps along K, so the activations of a
+//    step are read once per CTA.  The order of all additions depends on K alone: a
 //    row's bits depend neither on M nor on the other rows.
 //  * Both come in boxes of 128 bytes a row with the 128-byte swizzle (narrower
 //    rows, laid out for the reads, made the TMA unit the bound: it takes rows
@@ -46,14 +46,14 @@
 namespace tg {
 
 namespace gemv4 {
-constexpr int WK = 4;                 // warps along K = blocks of 128 codes per step
+constexpr int WK = 4;                 // warps along K
 constexpr int MAX_STAGES = 16;
 __host__ __device__ constexpr int threads(int wr) { return 32 * (WK * wr + 1); }
 __host__ __device__ constexpr int rows(int rt, int wr) { return 16 * rt * wr; }
 // Bytes of a ring slot's weights ([two blocks][row][128]) and activations
-// ([block][row][128]), and of the scales of the CTA's rows.
-__host__ __device__ constexpr uint32_t w_bytes(int rows) { return uint32_t(rows) * WK * 64; }
-__host__ __device__ constexpr uint32_t x_bytes(int m) { return (uint32_t(m) * WK * 128 + 1023u) & ~1023u; }
+// ([block][row][128]) with kb blocks a warp, and of the scales of the CTA's rows.
+__host__ __device__ constexpr uint32_t w_bytes(int kb, int rows) { return uint32_t(kb * rows) * WK * 64; }
+__host__ __device__ constexpr uint32_t x_bytes(int kb, int m) { return (uint32_t(kb * m) * WK * 128 + 1023u) & ~1023u; }
 __host__ __device__ constexpr uint32_t scale_bytes(int rows, int groups, bool s4) {
   return (uint32_t(rows) * uint32_t(groups) * (s4 ? 4u : 2u) + 15u) & ~15u;
 }
@@ -152,16 +152,17 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 }
 
 // MT: activation rows padded to 8 MT; RT: row tiles of 16 weights per warp; WR:
-// warps along N; SV: scales per block of 128 codes (groups of 32: 4, 64: 2, 128
-// and 256: 1); S4: fp32 scales.
-template <int MT, int RT, int WR, int SV, bool S4>
+// warps along N; KB: blocks of 128 codes a warp takes per step; SV: scales per block
+// (groups of 32: 4, 64: 2, 128 and 256: 1); S4: fp32 scales.
+template <int MT, int RT, int WR, int KB, int SV, bool S4>
 __global__ void __launch_bounds__(gemv4::threads(WR), 1)
     gemv_i4_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                    const GemvI4Params p) {
   using namespace gemv4;
   constexpr int THREADS = threads(WR);
   constexpr int ROWS = rows(RT, WR), COLS = MT * 8;
-  constexpr uint32_t W_BYTES = w_bytes(ROWS);
+  constexpr int STEP = KB * WK;  // blocks per step
+  constexpr uint32_t W_BYTES = w_bytes(KB, ROWS);
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
   constexpr bool CONVERT = MT == 8 && SV >= 2;
   // Ring slots [weights | activations], then the scales; the partial tiles of the
@@ -176,8 +177,8 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * ROWS;
   const int blocks = p.K / 128;
-  const int steps = (blocks + WK - 1) / WK;
-  const uint32_t slot_bytes = W_BYTES + x_bytes(p.M);
+  const int steps = (blocks + STEP - 1) / STEP;
+  const uint32_t slot_bytes = W_BYTES + x_bytes(KB, p.M);
   // The scales of this CTA's rows are one stretch of wscale (16-byte aligned: n0 is
   // a multiple of 16); its last bytes may not fill 16.
   constexpr uint32_t SSZ = S4 ? 4 : 2;
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
     fence_mbar_init();
     abort_flag = 0;
     // Only into L2: the kernel before may be the one that wrote the weight.
-    for (int s = 0; s < (WK / 2) * p.prefetch; ++s) tma_prefetch_l2_2d(&tma_w, s * 128, n0);
+    for (int s = 0; s < (STEP / 2) * p.prefetch; ++s) tma_prefetch_l2_2d(&tma_w, s * 128, n0);
   }
   __syncthreads();
   pdl_wait();
@@ -236,11 +237,11 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
       for (int s = 0; s < steps; ++s) {
         if (!wait(&empty_bar[slot], phase ^ 1u, DEVERR_PIPE_TIMEOUT)) break;
         uint8_t* dst = smem4 + uint32_t(slot) * slot_bytes;
-        mbar_arrive_expect_tx(&full_bar[slot], W_BYTES + uint32_t(p.M) * (WK * 128));
+        mbar_arrive_expect_tx(&full_bar[slot], W_BYTES + uint32_t(p.M) * (STEP * 128));
 #pragma unroll
-        for (int b = 0; b < WK / 2; ++b)
-          tma_load_2d(dst + b * (ROWS * 128), &tma_w, &full_bar[slot], (s * (WK / 2) + b) * 128, n0);
-        tma_load_3d(dst + W_BYTES, &tma_x, &full_bar[slot], 0, 0, s * WK);
+        for (int b = 0; b < STEP / 2; ++b)
+          tma_load_2d(dst + b * (ROWS * 128), &tma_w, &full_bar[slot], (s * (STEP / 2) + b) * 128, n0);
+        tma_load_3d(dst + W_BYTES, &tma_x, &full_bar[slot], 0, 0, s * STEP);
         ++filled;
         if (++slot == p.stages) {
           slot = 0;
@@ -264,11 +265,14 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
                                     ((((kw & 1) * 4 + t) ^ w_row(g)) << 4));
     // (Rows from M up are whatever lies behind: their columns are dropped.)  A row's
     // swizzle follows from its place in the slot.
-    const int xr = kw * p.M + x_row(g);
-    uint32_t x_off[4];
+    uint32_t x_off[KB][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x_off[j] = W_BYTES + uint32_t(xr * 128 + (((2 * j + (t >> 1)) ^ (xr & 7)) << 4) + (t & 1) * 8);
+    for (int k = 0; k < KB; ++k) {
+      const int xr = (k * WK + kw) * p.M + x_row(g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x_off[k][j] = W_BYTES + uint32_t(xr * 128 + (((2 * j + (t >> 1)) ^ (xr & 7)) << 4) + (t & 1) * 8);
+    }
     // (The rows past N read whatever lies behind the scales: they are dropped.)
     const uint32_t spitch = uint32_t(p.groups) * SSZ;
     const uint8_t* srow = scale + uint32_t(wr * RT * 16 + w_row(g)) * spitch;
@@ -284,67 +288,71 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
     const bool go = __all_sync(0xffffffffu, wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT));
     for (int s = 0; go && s < steps; ++s) {
       if (!__all_sync(0xffffffffu, wait(&full_bar[slot], phase, DEVERR_TMA_TIMEOUT))) break;
-      const int b = s * WK + kw;
-      if (b < blocks) {
-        const uint8_t* base = smem4 + uint32_t(slot) * slot_bytes;
-        uint4 w[RT][2];
-        float sc[RT][2][SV];
-        const uint32_t si = uint32_t(b >> p.scale_shift) * (SV * SSZ);
+      const uint8_t* base = smem4 + uint32_t(slot) * slot_bytes;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+      for (int k = 0; k < KB; ++k) {
+        const int b = s * STEP + k * WK + kw;
+        if (b < blocks) {
+          uint4 w[RT][2];
+          float sc[RT][2][SV];
+          const uint32_t si = uint32_t(b >> p.scale_shift) * (SV * SSZ);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            w[r][h] = *reinterpret_cast<const uint4*>(base + w_off + (r * 16 + h * 8) * 128);
-            RawScale<SV, S4> raw;
-            raw.load(srow + (r * 16 + h * 8) * spitch + si);
+          for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int i = 0; i < SV; ++i) sc[r][h][i] = raw.get(i, f16);
-          }
-        uint32_t lo[RT][2][4], hi[RT][2][4];
+            for (int h = 0; h < 2; ++h) {
+              w[r][h] = *reinterpret_cast<const uint4*>(base + w_off + (k * (WK / 2) * ROWS + r * 16 + h * 8) * 128);
+              RawScale<SV, S4> raw;
+              raw.load(srow + (r * 16 + h * 8) * spitch + si);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t v[4] = {w[r][h].x, w[r][h].y, w[r][h].z, w[r][h].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
-              hi[r][h][j] = v[j] & 0xf0f0f0f0u;
+              for (int i = 0; i < SV; ++i) sc[r][h][i] = raw.get(i, f16);
             }
+          uint32_t lo[RT][2][4], hi[RT][2][4];
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t v[4] = {w[r][h].x, w[r][h].y, w[r][h].z, w[r][h].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                lo[r][h][j] = (v[j] << 4) & 0xf0f0f0f0u;
+                hi[r][h][j] = v[j] & 0xf0f0f0f0u;
+              }
+            }
+          // IB column tiles at a time, all their products first: a product's result
+          // takes about 35 cycles, so neighbouring ones must not wait for each other.
+          constexpr int IB = MT >= 2 && SV <= 2 ? 2 : 1;
+          constexpr int MM = 4 / SV;  // products per scale
+#pragma unroll
+          for (int i0 = 0; i0 < MT; i0 += IB) {
+            uint2 x[IB][4];
+#pragma unroll
+            for (int i = 0; i < IB; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                x[i][j] = *reinterpret_cast<const uint2*>(base + x_off[k][j] + (i0 + i) * 1024);
+            int v[IB][RT][SV][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < IB; ++i)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                  int(&d)[4] = v[i][r][j / MM];
+                  if (j % MM == 0) mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], magic);
+                  else mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], d);
+                }
+#pragma unroll
+            for (int q = 0; q < SV; ++q)
+#pragma unroll
+              for (int i = 0; i < IB; ++i)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                  const int(&d)[4] = v[i][r][q];
+                  float2(&o)[2] = acc[r][i0 + i];
+                  o[0] = fma2(sums(d[0], d[1]), make_float2(sc[r][0][q], sc[r][0][q]), o[0]);
+                  o[1] = fma2(sums(d[2], d[3]), make_float2(sc[r][1][q], sc[r][1][q]), o[1]);
+                }
           }
-        // IB column tiles at a time, all their products first: a product's result
-        // takes about 35 cycles, so neighbouring ones must not wait for each other.
-        constexpr int IB = MT >= 2 && SV <= 2 ? 2 : 1;
-        constexpr int MM = 4 / SV;  // products per scale
-#pragma unroll
-        for (int i0 = 0; i0 < MT; i0 += IB) {
-          uint2 x[IB][4];
-#pragma unroll
-          for (int i = 0; i < IB; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = *reinterpret_cast<const uint2*>(base + x_off[j] + (i0 + i) * 1024);
-          int v[IB][RT][SV][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < IB; ++i)
-#pragma unroll
-              for (int r = 0; r < RT; ++r) {
-                int(&d)[4] = v[i][r][j / MM];
-                if (j % MM == 0) mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], magic);
-                else mma_s8(d, lo[r][0][j], lo[r][1][j], hi[r][0][j], hi[r][1][j], x[i][j], d);
-              }
-#pragma unroll
-          for (int q = 0; q < SV; ++q)
-#pragma unroll
-            for (int i = 0; i < IB; ++i)
-#pragma unroll
-              for (int r = 0; r < RT; ++r) {
-                const int(&d)[4] = v[i][r][q];
-                float2(&o)[2] = acc[r][i0 + i];
-                o[0] = fma2(sums(d[0], d[1]), make_float2(sc[r][0][q], sc[r][0][q]), o[0]);
-                o[1] = fma2(sums(d[2], d[3]), make_float2(sc[r][1][q], sc[r][1][q]), o[1]);
-              }
         }
       }
       __syncwarp();
