@@ -247,7 +247,7 @@ int tg_int4_gemv_dequant(const int8_t *xq, const float *xscale, const uint8_t *w
  * No reference counterpart, nor have the three functions below.
  *
  *   logits   [T, E] of dtype (TG_DT_F32/F16/BF16); E <= TG_MAX_EXPERTS,
- *            top_k <= min(E, TG_MAX_TOP_K)
+ *            top_k <= min(E, TG_MAX_TOP_K), T * top_k <= 2^30
  *   ids      [T, top_k] out: the experts of the largest logits, descending;
  *            equal logits by ascending index, NaN above everything
  *   weights  [T, top_k] fp32 out: exp(l - l_max) / sum, the sum over the

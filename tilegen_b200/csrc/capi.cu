@@ -1293,7 +1293,7 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
                      size_t workspace_bytes, void* stream) {
   if (T < 0 || E <= 0 || top_k <= 0 || top_k > E || !is_dtype(dtype)) return TG_ERR_INVALID_ARG;
   if (E > tg::route::MAX_E || top_k > tg::route::MAX_K) return TG_ERR_UNSUPPORTED;
-  if (T * top_k >= (int64_t(1) << 31)) return TG_ERR_UNSUPPORTED;
+  if (T > (int64_t(1) << 30) / top_k) return TG_ERR_UNSUPPORTED;  // 32-bit slot numbers, with room for a grid's stride
   if (!offsets || !aligned_to(offsets, 4)) return offsets ? TG_ERR_MISALIGNED : TG_ERR_INVALID_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0)

@@ -457,7 +457,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
         raise ValueError(f"{fn}: {e} experts, 1 to {MAX_EXPERTS} are supported")
     if not 1 <= top_k <= min(e, MAX_TOP_K):
         raise ValueError(f"{fn}: top_k={top_k} must be 1 to {min(e, MAX_TOP_K)}")
-    if t * top_k >= 1 << 31:
+    if t * top_k > 1 << 30:
         raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
     _no_grad(fn, logits)
     logits = logits.contiguous()
