@@ -1116,7 +1116,7 @@ uint32_t gemv4_smem(int m, int mt, int rows, int kb, int groups, bool s4, int st
   using namespace tg::gemv4;
   const uint32_t ring = uint32_t(stages) * (w_bytes(kb, rows) + x_bytes(kb, m));
   return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) +
-         2048u;  // alignment, and what the reads of rows past m may overrun
+         1024u + uint32_t(8 * mt - m) * 128u;  // alignment, and the rows past m that are read and dropped
 }
 
 // want: CTAs per SM to make room for; as many ring slots as then fit (two at least).

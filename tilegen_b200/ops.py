@@ -61,9 +61,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
 
-# An uninitialised tensor on the current device, without the dispatcher's round
-# (0.7 us where torch.empty takes 1.6), where torch has the allocator entry its
-# own generated code uses.
+# (shape, stride, dtype) -> an uninitialised tensor on the current device, without
+# the dispatcher's round (0.7 us where torch.empty takes 1.6), where torch has the
+# allocator entry that its own generated code uses.
 _fast_empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
@@ -461,11 +461,13 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
         raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
     _no_grad(fn, logits)
     logits = logits.contiguous()
-    i32 = torch.int32
-    ids, weights, place = (_empty(dev, dt, t, top_k) for dt in (i32, torch.float32, i32))
-    offsets, rows = _empty(dev, i32, e + 1), _empty(dev, i32, t * top_k)
+    empty = _fast_empty if _fast_empty is not None and dev.index == torch.cuda.current_device() else (
+        lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=dev))
+    slots, stride, i32 = (t, top_k), (top_k, 1), torch.int32
+    ids, place, weights = empty(slots, stride, i32), empty(slots, stride, i32), empty(slots, stride, torch.float32)
+    offsets, rows = empty((e + 1,), (1,), i32), empty((t * top_k,), (1,), i32)
     need = _lib.lib().tg_route_experts_workspace(t, e)
-    work = _empty(dev, torch.uint8, need) if need else None
+    work = empty((need,), (1,), torch.uint8) if need else None
     _call("tg_route_experts", dev, logits.data_ptr(), _DTYPE_CODE[logits.dtype], t, e, top_k, 1 if renormalize else 0,
           weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), rows.data_ptr(), place.data_ptr(),
           work.data_ptr() if need else None, need)
