@@ -24,7 +24,7 @@
 //    flight share their weight rows in L2.  An expert without rows has no tile.
 //  * Activation rows come by TMA, XBOX rows a box, or with `rows` by
 //    tile::gather4 (box one row high).  One lane issuing a gather takes about 50
-//    cycles, so eight warps share them.
+//    cycles, so seven warps share them.
 //  * The epilogue holds one output channel per lane and a row per column: it
 //    stages 32 rows x 32 channels a warp in shared memory for one TMA store, and
 //    stores the part-filled last chunk of a group directly, row by row.
@@ -45,10 +45,10 @@ constexpr int STEP = 32;                 // granularity of the pair MMA's N
 constexpr int BK = 128;                  // bytes of K per k-block
 constexpr int UK = 32;                   // K per tcgen05.mma kind::i8
 constexpr uint32_t W_BYTES = BNW * BK;   // 16 KB
-constexpr int HELPERS = 7;               // producer warps beside warp 0 (gathered rows)
+constexpr int GATHERERS = 7;             // warps that gather rows, beside warp 0 (the weights)
 constexpr int STAGE_OUT = 4096;          // epilogue staging bytes per warp
 constexpr int MAX_E = TG_MAX_EXPERTS;
-__host__ __device__ constexpr int threads(bool gather) { return 192 + (gather ? 32 * HELPERS : 0); }
+__host__ __device__ constexpr int threads(bool gather) { return 192 + (gather ? 32 * GATHERERS : 0); }
 constexpr int XBOX = 32;                 // activation rows per TMA box
 // 128-byte K sub-blocks per ring slot (two, as gemm_i8.cuh's pairs), bytes of a
 // sub-block's activation rows in each CTA (half of the tile's), of a slot, ring depth.
@@ -234,13 +234,10 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
 
   if (warp == 0 || warp >= 6) {
     // ------------------------------------------------------------ producers
-    // Warp 0 loads the weight rows and announces the bytes.  Activation rows:
-    // by warp 0 in boxes, or gathered, each producer warp a quarter of them.
-    constexpr int XR = int(X_BYTES) / BK;             // activation rows of this CTA at most
-    constexpr int PRODUCERS = 1 + HELPERS;
-    constexpr int Q = (XR / 4 + PRODUCERS - 1) / PRODUCERS;  // gathers per warp at most
-    static_assert(Q <= 32, "one gather per lane");
-    const int part = warp == 0 ? 0 : warp - 5;
+    // Warp 0 loads the weight rows and announces the bytes; it also loads the
+    // activation rows in boxes.  Gathered ones are the other warps', so that the
+    // weights' loads never wait for row numbers.
+    static_assert(int(X_BYTES) / BK / 4 <= 32 * GATHERERS, "one gather per lane");
     int stage = 0, n_issued = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -251,11 +248,11 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
       const int first = int(rank) * mine;             // the first of them in the tile
       const int loaded = GATHER ? mine : (mine + XBOX - 1) / XBOX * XBOX;
       const uint32_t tx = 2u * uint32_t(KS) * (W_BYTES + uint32_t(loaded) * BK);
-      // This lane's gather: rows 4 (part + PRODUCERS lane) + 0..3 of this CTA's.
+      // This lane's gather: rows 4 (warp - 6 + GATHERERS lane) + 0..3 of this CTA's.
       // A row number outside xq reads row 0 (its scale is taken as 0).
-      const int gr = 4 * (part + PRODUCERS * lane);
+      const int gr = GATHER && warp != 0 ? 4 * (warp - 6 + GATHERERS * lane) : mine;
       int4 idx = make_int4(0, 0, 0, 0);
-      if (GATHER && gr < mine) {
+      if (gr < mine) {
         int v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -287,7 +284,7 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
           }
         }
         __syncwarp();
-        if (GATHER && gr < mine) {
+        if (gr < mine) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
             tma_gather4_pair(sx + ks * X_BYTES + gr * BK, &tma_x, fb, (kb * KS + ks) * BK, idx);
