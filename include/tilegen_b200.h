@@ -7,8 +7,9 @@
  *     synchronisation, no allocation;
  *   - returns a tg_status; nothing is launched when it is not TG_OK.
  * tg_rotate_quant, tg_quantize_act, tg_int8_gemm_dequant,
- * tg_int8_gemm_dequant_splitk and tg_int8_gemv_dequant work only on buffers
- * the caller owns, so they can be captured in CUDA graphs.
+ * tg_int8_gemm_dequant_splitk, tg_int8_gemv_dequant, tg_int4_gemv_dequant,
+ * tg_route_experts, tg_int8_grouped_gemm_dequant and tg_combine_experts work
+ * only on buffers the caller owns, so they can be captured in CUDA graphs.
  * Device-side failures (a bounded wait that gave up) are recorded in a device
  * status word that tg_device_status() reads.
  *

@@ -9,10 +9,15 @@ few-row GEMV on the CUDA cores; with up to ``SPLITK_MAX_M`` rows (see
 ``splitk_route``) the split-K kernel and a cached, self-clearing scratch per
 (device, stream); otherwise the tiled tcgen05 kernel.
 
+Beside them stand the linear's other weight forms: ``int4_gemv_dequant`` (4-bit weights
+with group scales, few rows) and the routed experts' ``route_experts``,
+``int8_grouped_gemm_dequant`` and ``combine_experts``.
+
 The same functions are registered as ``torch.ops.tilegen.rotate_quant``,
-``torch.ops.tilegen.quantize_act``, ``torch.ops.tilegen.quantize_ln_mod`` and
-``torch.ops.tilegen.int8_gemm_dequant``
-(with fake implementations, so they trace under ``torch.compile``/``torch.export``
+``torch.ops.tilegen.quantize_act``, ``torch.ops.tilegen.quantize_ln_mod``,
+``torch.ops.tilegen.int8_gemm_dequant``, ``torch.ops.tilegen.int4_gemv_dequant``,
+``torch.ops.tilegen.route_experts``, ``torch.ops.tilegen.int8_grouped_gemm_dequant``
+and ``torch.ops.tilegen.combine_experts`` (with fake implementations, so they trace under ``torch.compile``/``torch.export``
 as opaque ops).
 """
 from __future__ import annotations
