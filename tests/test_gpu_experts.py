@@ -491,6 +491,52 @@ def test_layer_in_a_graph_and_on_another_stream(cuda):
     del graph, second
 
 
+def test_layer_empty_padded_and_refusals(cuda):
+    e, k, f = 4, 256, 512
+    up, down = _layer(e, k, f, 5, torch.float16, cuda)
+    x, logits = torch.randn(2, 3, k, device=cuda).half(), torch.randn(2, 3, e, device=cuda)
+    assert int8_expert_ffn(x[:0], logits[:0], up, down, 2).shape == (0, 3, k)
+    closed = torch.full_like(logits, -math.inf)
+    assert (int8_expert_ffn(x, closed, up, down, 2) == 0).all()
+    assert torch.equal(int8_expert_ffn(x, closed, up, down, 2, residual=x), x)
+    # a padded token leaves the others as they are
+    y = int8_expert_ffn(x, logits, up, down, 2)
+    logits[1, 1] = -math.inf
+    z = int8_expert_ffn(x, logits, up, down, 2)
+    assert (z[1, 1] == 0).all()
+    keep = torch.ones(2, 3, dtype=torch.bool, device=cuda)
+    keep[1, 1] = False
+    assert torch.equal(y[keep], z[keep])
+    for bad in ((x.clone().requires_grad_(), logits, None), (x, logits.clone().requires_grad_(), None), (x, logits, x.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="gradient"):
+            int8_expert_ffn(bad[0], bad[1], up, down, 2, residual=bad[2])
+
+
+def test_layers_on_two_streams_at_once(cuda):
+    """Layers in flight together on two streams share nothing."""
+    up, down = _layer(8, 512, 768, 6, torch.bfloat16, cuda)
+    xs = [torch.randn(t, 512, generator=_gen(t), device=cuda).bfloat16() for t in (300, 7)]
+    ls = [torch.randn(t, 8, generator=_gen(t + 1), device=cuda) for t in (300, 7)]
+    want = [int8_expert_ffn(x, l, up, down, 2, residual=x) for x, l in zip(xs, ls)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(int8_expert_ffn(xs[i], ls[i], up, down, 2, residual=xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_grouped_with_few_sms(cuda):
+    """The SM budget's smallest grids still cover every tile."""
+    case = _group_case([300, 0, 5, 40], 520, 512, 60, seed=3)
+    for sms in (1, 2, 3, 100):
+        with ops.sm_budget(sms):
+            _check_group(case, torch.float16)
+
+
 def test_custom_ops(cuda):
     x = torch.randn(9, 8, generator=_gen(1), device=cuda)
     a, b = torch.ops.tilegen.route_experts(x, 2, True), ops.route_experts(x, 2)

@@ -189,6 +189,45 @@ def test_linear_against_the_rotated_product(cuda, m):
     _check(y[0], xq, xs, unpack_int4(w4), ws, bias)
 
 
+def test_linear_empty_and_refusals(cuda):
+    w4, ws = quantize_convrot_weight_int4(torch.randn(64, 256, device=cuda))
+    x = torch.randn(3, 256, device=cuda).half()
+    assert int4_linear(x[:0], w4, ws).shape == (0, 64)
+    with pytest.raises(ValueError, match="gradient"):
+        int4_linear(x.clone().requires_grad_(), w4, ws)
+    with torch.no_grad():
+        assert torch.equal(int4_linear(x.clone().requires_grad_(), w4, ws), int4_linear(x, w4, ws))
+    with pytest.raises(ValueError):
+        int4_linear(x.float(), w4, ws)
+
+
+@pytest.mark.parametrize("m", [1, 9, 17, 33, 40, 61, 64])
+def test_short_rows_that_are_not_a_multiple_of_eight(cuda, m):
+    """One block of K: the last slot's reads reach past the rows there are."""
+    for n, group in ((5, 128), (200, 32)):
+        xq, xs, codes, ws, bias = _case(m, n, 128, group, torch.float16, torch.float32, seed=m)
+        _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, torch.float32), xq, xs, codes, ws, bias)
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    """Calls in flight together on two streams share nothing."""
+    case = _case(12, 2000, 4096, 128, seed=8)
+    other = _case(50, 1500, 4096, 64, seed=9)
+    w4, o4 = pack_int4(case[2]), pack_int4(other[2])
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    ys, zs = [], []
+    for _ in range(20):
+        with torch.cuda.stream(a):
+            ys.append(ops.int4_gemv_dequant(case[0], case[1], w4, case[3], None, torch.float32))
+        with torch.cuda.stream(b):
+            zs.append(ops.int4_gemv_dequant(other[0], other[1], o4, other[3], None, torch.float32))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, ys[0]) for y in ys) and all(torch.equal(z, zs[0]) for z in zs)
+    _check(ys[0], *case[:4], None)
+    _check(zs[0], *other[:4], None)
+
+
 def test_custom_op(cuda):
     xq, xs, codes, ws, _ = _case(4, 32, 256, 64)
     w4 = pack_int4(codes)

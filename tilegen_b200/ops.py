@@ -17,8 +17,8 @@ The same functions are registered as ``torch.ops.tilegen.rotate_quant``,
 ``torch.ops.tilegen.quantize_act``, ``torch.ops.tilegen.quantize_ln_mod``,
 ``torch.ops.tilegen.int8_gemm_dequant``, ``torch.ops.tilegen.int4_gemv_dequant``,
 ``torch.ops.tilegen.route_experts``, ``torch.ops.tilegen.int8_grouped_gemm_dequant``
-and ``torch.ops.tilegen.combine_experts`` (with fake implementations, so they trace under ``torch.compile``/``torch.export``
-as opaque ops).
+and ``torch.ops.tilegen.combine_experts`` (with fake implementations, so they
+trace under ``torch.compile``/``torch.export`` as opaque ops).
 """
 from __future__ import annotations
 
@@ -360,7 +360,7 @@ def _on(fn: str, name: str, t, dev: torch.device, dtypes, ndim: int) -> None:
     raise ValueError(f"{fn}: {name} must be {ndim}-D of {' / '.join(map(str, dtypes))}, got {tuple(t.shape)} {t.dtype}")
 
 
-def _no_grad(fn: str, *tensors) -> None:
+def no_gradient(fn: str, *tensors) -> None:
     """The forms for serving have no backward pass: an input that wants a gradient is refused."""
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
@@ -422,7 +422,7 @@ def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, 
             raise ValueError(f"{fn}: bias has {bias.shape[0]} elements, expected {n}")
         bias = bias.contiguous()
         b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
-    _no_grad(fn, xscale, wscale, bias)
+    no_gradient(fn, xscale, wscale, bias)
     xq, w4, xscale, wscale = _aligned(xq), _aligned(w4), xscale.contiguous(), _aligned(wscale)
     out = _out(fn, out, (m, n), out_dtype, dev)
     if m:
@@ -464,7 +464,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
         raise ValueError(f"{fn}: top_k={top_k} must be 1 to {min(e, MAX_TOP_K)}")
     if t * top_k > 1 << 30:
         raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
-    _no_grad(fn, logits)
+    no_gradient(fn, logits)
     logits = logits.contiguous()
     empty = _fast_empty if _fast_empty is not None and dev.index == torch.cuda.current_device() else (
         lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=dev))
@@ -529,7 +529,7 @@ def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.
         _on(fn, "rows", rows, dev, _I32, 1)
         rows = rows.contiguous()
         r, r_ptr = rows.shape[0], rows.data_ptr()
-    _no_grad(fn, xscale, wscale, bias)
+    no_gradient(fn, xscale, wscale, bias)
     xq, wq = _aligned(xq), _aligned(wq)
     xscale, wscale, offsets = xscale.contiguous(), wscale.contiguous(), offsets.contiguous()
     out = _out(fn, out, (r, n), out_dtype, dev)
@@ -571,7 +571,7 @@ def combine_experts(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor,
         if tuple(residual.shape) != (t, n):
             raise ValueError(f"{fn}: residual is {tuple(residual.shape)}, expected {(t, n)}")
         residual = residual.contiguous()
-    _no_grad(fn, y, weights, residual)
+    no_gradient(fn, y, weights, residual)
     y, place, weights = y.contiguous(), place.contiguous(), weights.contiguous()
     out = _out(fn, out, (t, n), y.dtype, dev, y.element_size())
     if t:

@@ -38,6 +38,7 @@ def int8_expert_ffn(x: torch.Tensor, logits: torch.Tensor, up, down, top_k: int,
         raise ValueError(f"logits {tuple(logits.shape)} do not match x {tuple(x.shape)}")
     if down[0].shape[1] != k:
         raise ValueError(f"down projects to {down[0].shape[1]} channels, x has {k}")
+    ops.no_gradient("int8_expert_ffn", x, logits, residual)
     routes = ops.route_experts(logits.reshape(-1, logits.shape[-1]), top_k, renormalize)
     xq, xscale = ops.rotate_quant(x2, group_size)
     h = ops.int8_grouped_gemm_dequant(xq, xscale, up[0], up[1], up[2], routes.offsets, x.dtype, rows=routes.rows)

@@ -82,6 +82,7 @@ def int4_linear(x: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor, bias: t
     k = x.shape[-1]
     if k != w4.shape[-1] * 2:
         raise ValueError(f"input and weight inner dimensions differ: {k} != {w4.shape[-1] * 2}")
+    ops.no_gradient("int4_linear", x)
     out_dtype = out_dtype or x.dtype
     xq, xscale = ops.quantize_act(x.reshape(-1, k), group_size, input_act)
     m, n = xq.shape[0], w4.shape[0]
