@@ -225,8 +225,9 @@ int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
  *   out[m,n] = (sum_g wscale[n,g] * float(sum_{k in g} xq[m,k] * w4[n,k])) * xscale[m] + bias[n]
  *
  * The inner sums are exact (a group of 256: each half's), the outer one is fp32
- * in an order that depends on K only (a row's result does not depend on the
- * other rows or on M).
+ * in an order of its own for M == 1 (a kernel for one row) and in one that
+ * depends on K only from M == 2 up: there a row's result depends neither on the
+ * other rows nor on M.
  *
  *   xq      [M, K] int8, 16-B aligned; K % 128 == 0, K at most
  *           tg_rotate_quant_max_k()

@@ -52,7 +52,7 @@ def _check(y, xq, xs, codes, ws, bias):
 
 
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
-@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 33, 64])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 33, 64])
 def test_rows_and_groups(cuda, m, group):
     xq, xs, codes, ws, bias = _case(m, 200, 768, group, seed=m)
     _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, torch.float32), xq, xs, codes, ws, bias)
@@ -62,7 +62,7 @@ def test_rows_and_groups(cuda, m, group):
 @pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("bias_dtype", [None, torch.float32, torch.float16, torch.bfloat16])
 def test_types(cuda, out_dtype, scale_dtype, bias_dtype):
-    for m in (1, 12):
+    for m in (1, 3, 12):
         xq, xs, codes, ws, bias = _case(m, 130, 512, 64, scale_dtype, bias_dtype, seed=3)
         _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, out_dtype), xq, xs, codes, ws, bias)
 
@@ -70,7 +70,7 @@ def test_types(cuda, out_dtype, scale_dtype, bias_dtype):
 @pytest.mark.parametrize("n,k,group", [(1, 128, 32), (1, 128, 128), (15, 128, 64), (16, 256, 256), (17, 1408, 128), (33, 14080, 128),
                                        (1001, 5120, 32), (5120, 13824, 256), (13823, 5120, 128)])
 def test_odd_and_block_shapes(cuda, n, k, group):
-    for m in (1, 5, 40):
+    for m in (1, 2, 4, 5, 40):
         xq, xs, codes, ws, bias = _case(m, n, k, group, torch.bfloat16, torch.float16, seed=n + k + m)
         _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, torch.bfloat16), xq, xs, codes, ws, bias)
 
@@ -78,32 +78,37 @@ def test_odd_and_block_shapes(cuda, n, k, group):
 def test_extreme_codes_do_not_overflow(cuda):
     """-128 times -8 over the largest K the group allows: the int32 sums and 16-fold codes hold them."""
     k = 32768
-    xq = torch.full((3, k), -128, dtype=torch.int8, device=cuda)
     codes = torch.full((16, k), -8, dtype=torch.int8, device=cuda)
     ws = torch.full((16, k // 256), 1.0, device=cuda)
-    y = ops.int4_gemv_dequant(xq, torch.ones(3, device=cuda), pack_int4(codes), ws, None, torch.float32)
-    assert (y == 1024.0 * k).all()  # every partial sum is a multiple of 2^10, at most 2^25: exact
+    for m in (1, 4, 5, 64):
+        xq = torch.full((m, k), -128, dtype=torch.int8, device=cuda)
+        y = ops.int4_gemv_dequant(xq, torch.ones(m, device=cuda), pack_int4(codes), ws, None, torch.float32)
+        assert (y == 1024.0 * k).all()  # every partial sum is a multiple of 2^10, at most 2^25: exact
 
 
 def test_a_row_does_not_depend_on_the_others(cuda):
-    """Row i of a batch has the bits of that row alone."""
+    """Row i has the same bits in every batch of two rows or more, and one row alone the same wherever it comes from."""
     xq, xs, codes, ws, _ = _case(64, 333, 2048, 128, seed=5)
     w4 = pack_int4(codes)
     y = ops.int4_gemv_dequant(xq, xs, w4, ws, None, torch.float32)
-    for rows in ((0, 1), (3, 5), (10, 19), (40, 64), (31, 48)):
-        a = ops.int4_gemv_dequant(xq[rows[0]:rows[1]], xs[rows[0]:rows[1]], w4, ws, None, torch.float32)
-        assert torch.equal(a, y[rows[0]:rows[1]])
+    for i, j in ((0, 2), (1, 3), (3, 5), (3, 8), (10, 19), (40, 64), (31, 48), (0, 33)):
+        assert torch.equal(ops.int4_gemv_dequant(xq[i:j], xs[i:j], w4, ws, None, torch.float32), y[i:j])
+    one = [ops.int4_gemv_dequant(q[i:i + 1], xs[i:i + 1], w4, ws, None, torch.float32)
+           for q, i in ((xq, 7), (xq.clone(), 7))]
+    assert torch.equal(one[0], one[1])
+    _check(one[0], xq[7:8], xs[7:8], codes, ws, None)
 
 
 def test_infinite_and_nan_scales_stay_in_their_row(cuda):
-    xq, xs, codes, ws, _ = _case(4, 64, 512, 128, torch.float32, seed=6)
-    ws[3, 1] = float("inf")
-    ws[7, 0] = float("nan")
-    xs[2] = float("nan")
-    y = ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, None, torch.float32)
-    assert y[2].isnan().all() and y[:, 7].isnan().all() and not y[[0, 1, 3], 3].isfinite().any()
-    keep = [i for i in range(64) if i not in (3, 7)]
-    assert y[[0, 1, 3]][:, keep].isfinite().all()
+    for m in (4, 8):
+        xq, xs, codes, ws, _ = _case(m, 64, 512, 128, torch.float32, seed=6)
+        ws[3, 1] = float("inf")
+        ws[7, 0] = float("nan")
+        xs[2] = float("nan")
+        y = ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, None, torch.float32)
+        assert y[2].isnan().all() and y[:, 7].isnan().all() and not y[[0, 1, 3], 3].isfinite().any()
+        keep = [i for i in range(64) if i not in (3, 7)]
+        assert y[[0, 1, 3]][:, keep].isfinite().all()
 
 
 def test_strided_and_unaligned_inputs(cuda):
@@ -147,9 +152,10 @@ def test_weight_past_32_bit_offsets(cuda):
     w4[-24:] = pack_int4(codes)
     scale = torch.ones(n, k // 256, dtype=torch.float16, device=cuda)
     scale[-24:] = ws
-    y = ops.int4_gemv_dequant(xq, xs, w4, scale, None, torch.float32)
-    _check(y[:, -24:], xq, xs, codes, ws, None)
-    assert (y[:, :-24] == 0).all()
+    for q, s in ((xq, xs), (xq.repeat(3, 1), xs.repeat(3))):  # each kernel
+        y = ops.int4_gemv_dequant(q, s, w4, scale, None, torch.float32)
+        _check(y[:, -24:], q, s, codes, ws, None)
+        assert (y[:, :-24] == 0).all()
 
 
 def test_other_stream_and_graph(cuda):

@@ -1119,6 +1119,50 @@ uint32_t gemv4_smem(int m, int mt, int rows, int kb, int groups, bool s4, int st
          1024u + uint32_t(8 * mt - m) * 128u;  // alignment, and the rows past m that are read and dropped
 }
 
+// K parts per group of four weight rows, as gemv_parts: the fewest that put two
+// CTAs on every SM, each part keeping two chunks a lane.
+int gemv4_parts(int64_t N, int64_t K, int sms) {
+  using namespace tg::gemv4one;
+  const int64_t row_groups = (N + R - 1) / R, nch = K / 32;
+  int kp = 1;
+  while (kp < WARPS && (row_groups * kp + WARPS - 1) / WARPS < 2 * int64_t(sms) && nch >= int64_t(64) * kp) kp *= 2;
+  return kp;
+}
+
+template <int U, int SV, bool S4>
+int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, int dev, cudaStream_t st) {
+  static uint32_t attr_done[kMaxDevices];
+  auto kern = tg::gemv_i4_one_kernel<U, SV, S4>;
+  if (!ensure_smem_attr(kern, dev, uint32_t(kRotQuantMaxK), attr_done)) return TG_ERR_CUDA;
+  return launch_dependent(kern, p, dim3(unsigned(ctas)), tg::gemv4one::THREADS, uint32_t(p.K), st);
+}
+
+// Two chunks of a row under way at once need registers that leave three CTAs per
+// SM, and help where the launch is one wave of those and a lane has more than two
+// chunks; otherwise four CTAs per SM with one chunk each carry more.  Measured (K x
+// N, two / one, us): 13824 x 5120 8.6 / 10.1, 5120 x 5120 5.2 / 5.7; 5120 x 15360
+// (480 CTAs) 11.4 / 8.3, 2048 x 1536 (two chunks a lane) 2.35 / 2.15.  Groups of 32
+// with fp32 scales are 16 more registers a chunk, too many: 12.7 / 11.2.
+template <int SV, bool S4>
+int launch_gemv4_one_sv(const tg::GemvI4OneParams& p, int sms, int dev, cudaStream_t st) {
+  using namespace tg::gemv4one;
+  const int64_t row_groups = (int64_t(p.N) + R - 1) / R, per_cta = WARPS / p.kp;
+  const int64_t ctas = (row_groups + per_cta - 1) / per_cta;
+  if constexpr (SV < 4 || !S4) {
+    if (ctas <= 3 * int64_t(sms) && p.part_chunks > 64) return launch_gemv4_one_t<2, SV, S4>(p, ctas, dev, st);
+  }
+  return launch_gemv4_one_t<1, SV, S4>(p, ctas, dev, st);
+}
+
+int launch_gemv4_one(const tg::GemvI4OneParams& p, int sv, int sms, int dev, cudaStream_t st) {
+  const bool s4 = p.wscale_dtype == TG_DT_F32;
+  switch (sv) {
+    case 4: return s4 ? launch_gemv4_one_sv<4, true>(p, sms, dev, st) : launch_gemv4_one_sv<4, false>(p, sms, dev, st);
+    case 2: return s4 ? launch_gemv4_one_sv<2, true>(p, sms, dev, st) : launch_gemv4_one_sv<2, false>(p, sms, dev, st);
+    default: return s4 ? launch_gemv4_one_sv<1, true>(p, sms, dev, st) : launch_gemv4_one_sv<1, false>(p, sms, dev, st);
+  }
+}
+
 // want: CTAs per SM to make room for; as many ring slots as then fit (two at least).
 template <int MT, int RT, int WR, int KB, int SV, bool S4>
 int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int want, int dev, cudaStream_t st) {
@@ -1186,7 +1230,8 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (M == 0) return TG_OK;
   if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(w4) || !aligned16(wscale)) return TG_ERR_MISALIGNED;
-  if (!aligned_to(xscale, 4) || !aligned_to(out, dtype_bytes(out_dtype)) || (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
+  if (!aligned_to(xscale, 4) || !aligned_to(out, dtype_bytes(out_dtype)) ||
+      (bias && !aligned_to(bias, dtype_bytes(bias_dtype))))
     return TG_ERR_MISALIGNED;
   tg::GemvI4Params p;
   p.xscale = xscale;
@@ -1206,11 +1251,31 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (!current_device(&dev, &info)) return TG_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sv = group == 32 ? 4 : (group == 64 ? 2 : 1);
+  if (M == 1) {
+    tg::GemvI4OneParams q;
+    q.xq = xq;
+    q.xscale = xscale;
+    q.w4 = w4;
+    q.wscale = wscale;
+    q.bias = bias;
+    q.wscale_dtype = wscale_dtype;
+    q.bias_dtype = bias_dtype;
+    q.out_dtype = out_dtype;
+    q.groups = p.groups;
+    q.scale_shift = p.scale_shift;
+    q.N = p.N;
+    q.K = p.K;
+    q.kp = gemv4_parts(N, K, info.sms_all);
+    q.part_chunks = int((K / 32 + q.kp - 1) / q.kp);
+    q.prefetch = N * K / 2 <= kGemvPrefetchMaxBytes ? 1 : 0;
+    q.out = out;
+    return launch_gemv4_one(q, sv, info.sms_all, dev, st);
+  }
   // 16-row tiles an SM gets.  Where they are few, a CTA's steps are what takes the
   // time, and two blocks a step halve them; where they are many, one block a step
-  // leaves room for the rings of more CTAs.  Measured (two blocks / one, us): one
-  // row, 5120 x 5120 5.9 / 6.8, 5120 x 13824 13.6 / 14.7; 15360 x 5120 with 8 rows
-  // 14.0 / 9.6, with 16 rows 17.5 / 11.9.
+  // leaves room for the rings of more CTAs.  Measured (two blocks / one, us): 4 rows,
+  // K x N = 5120 x 5120 6.1 / 6.7, 13824 x 5120 13.5 / 13.4; 5120 x 15360 with 8
+  // rows 13.3 / 9.7, with 16 rows 14.0 / 12.1.
   const int64_t tiles = (N + 15) / 16, sms = info.sms_all;
   const int want = int(std::max<int64_t>(1, std::min<int64_t>(8, (tiles + sms - 1) / sms)));
   const bool few = want <= 3;

@@ -25,7 +25,7 @@
 //  * A CTA has WR * RT * 16 weight rows and all of K.  A step is one or two blocks
 //    of 128 codes for each of the four warps along K, so the activations of a
 //    step are read once per CTA.  The order of all additions depends on K alone: a
-//    row's bits depend neither on M nor on the other rows.
+//    row's bits depend neither on M (from two rows up) nor on the other rows.
 //  * Both come in boxes of 128 bytes a row with the 128-byte swizzle (narrower
 //    rows, laid out for the reads, made the TMA unit the bound: it takes rows
 //    at a fixed rate); a step's activations are one copy, by a
@@ -39,9 +39,23 @@
 //    subtraction and one paired fma per two outputs and group, no conversion.
 //    With 64 columns and several groups a block the conversions, on another
 //    pipe than the fmas, are the faster way (61 rows, groups of 32: 29 us, not 39).
+//
+// One activation row has a kernel of its own (gemv_i4_one_kernel): the matrix
+// instructions would use an eighth of their columns, and the ring's start-up and
+// steps are much of so short a launch.  Four weight rows per warp with plain
+// 128-bit loads and dp4a, as gemv_i8_kernel.  Lane l takes the 16-byte chunks l,
+// l + 32, ... of its part of K; a chunk holds 8 codes of each 32 of a block, so the
+// CTA first lays the row out in shared memory as [half][chunk][16 bytes], two
+// 128-bit reads a chunk that serve the four rows.  K x N, this form / the ring (us):
+// 2048 x 1536 2.2 / 2.9, 5120 x 15360 8.3 / 9.4, 5120 x 5120 5.3 / 5.3, 13824 x 5120
+// 8.6 / 11.5.  It is bound by the weight's latency (one wave of loads that depend on
+// the CTAs resident).  Written for more rows it took, with two rows, 13.1 us on
+// 5120 x 15360 and 11.8 on 13824 x 5120 (the ring 9.7 and 13.6), and with four 16.3
+// and 20.7 (the ring as with two).
 #pragma once
 
 #include "common.cuh"
+#include "gemv_i8.cuh"
 
 namespace tg {
 
@@ -114,7 +128,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 template <int SV, bool S4>
 struct RawScale {
   uint32_t v[S4 ? SV : (SV + 1) / 2];
-  __device__ __forceinline__ void load(const uint8_t* q) {
+  __device__ __forceinline__ void load(const uint8_t* q) {  // from shared or global memory
     constexpr int BYTES = SV * (S4 ? 4 : 2);
     if constexpr (BYTES == 2) {
       v[0] = *reinterpret_cast<const unsigned short*>(q);
@@ -391,6 +405,142 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
     v = v * 0.0625f * p.xscale[m];
     if (p.bias) v += load_as_f32(p.bias, p.bias_dtype, size_t(n));
     store_f32_as(p.out, p.out_dtype, size_t(m) * p.N + n, v);
+  }
+}
+
+// One row on the CUDA cores (the header says why and what it measured).
+namespace gemv4one {
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int R = 4;  // weight rows per warp
+}  // namespace gemv4one
+
+struct GemvI4OneParams {
+  const int8_t* xq;
+  const float* xscale;
+  const uint8_t* w4;
+  const void* wscale;   // [N, groups] of wscale_dtype
+  const void* bias;
+  int wscale_dtype;
+  int bias_dtype;
+  int out_dtype;
+  int groups;           // K / group
+  int scale_shift;      // groups of 256: 1 (two blocks share a scale), else 0
+  int N, K;
+  int kp;               // K parts per row group = warps per group (1, 2, 4 or 8)
+  int part_chunks;      // 16-byte chunks of a row per part
+  int prefetch;         // 1: prefetch a quarter of each warp's weight rows into L2 first
+  void* out;            // [1, N] of out_dtype
+};
+
+// U: chunks of each row that a lane has under way; SV, S4 as in gemv_i4_kernel.
+template <int U, int SV, bool S4>
+__global__ void __launch_bounds__(gemv4one::THREADS, U == 1 ? 4 : 3) gemv_i4_one_kernel(const GemvI4OneParams p) {
+  using namespace gemv4one;
+  constexpr int SSZ = S4 ? 4 : 2;
+  extern __shared__ __align__(16) uint8_t sx[];  // [2][chunks][16]
+  __shared__ float partial[WARPS][R];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kp = p.kp;
+  const int groups_per_cta = WARPS / kp;
+  const int g_local = warp / kp, part = warp - g_local * kp;
+  const uint32_t N = uint32_t(p.N);  // rows past the last one pass 2^31
+  const uint32_t n0 = (blockIdx.x * uint32_t(groups_per_cta) + uint32_t(g_local)) * R;
+  const int nch = p.K >> 5;
+  const int c0 = part * p.part_chunks;
+  const int c1 = min(c0 + p.part_chunks, nch);
+  const bool live = n0 < N && c0 < c1;
+  pdl_launch_dependents();
+  if (live && p.prefetch && lane < R && n0 + lane < N)
+    prefetch_l2_bulk(p.w4 + (size_t(n0 + lane) * size_t(nch) + size_t(c0)) * 16u, uint32_t(c1 - c0 + 3) / 4u * 16u);
+  pdl_wait();
+
+  // U chunks of the four rows and their scales (a row past N reads the last one's
+  // and is dropped; a chunk past the part's end its last one's).
+  const uint32_t first = min(n0, N - 1);
+  const uint8_t* const wbase = p.w4 + size_t(first) * (size_t(nch) * 16u);
+  const uint8_t* const sbase = static_cast<const uint8_t*>(p.wscale) + size_t(first) * (size_t(p.groups) * SSZ);
+  uint32_t wrow[R], srow[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t n = min(uint32_t(r), N - 1 - first);
+    wrow[r] = n * uint32_t(nch) * 16u;
+    srow[r] = n * uint32_t(p.groups) * SSZ;
+  }
+  int4 w[U][R];
+  RawScale<SV, S4> sc[U][R];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int cc = min(c + 32 * u, c1 - 1);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        w[u][r] = ld_stream_v4(reinterpret_cast<const int4*>(wbase + (wrow[r] + uint32_t(cc) * 16u)));
+        sc[u][r].load(sbase + (srow[r] + uint32_t((cc >> 2) >> p.scale_shift) * uint32_t(SV * SSZ)));
+      }
+    }
+  };
+  if (live) load(c0 + lane);  // under way while the activations are laid out
+  for (int q = threadIdx.x; q < p.K >> 4; q += THREADS) {  // 16 codes: two pieces
+    const int4 v = *reinterpret_cast<const int4*>(p.xq + q * 16);
+    const int j = (q >> 1) & 3, chunk = (q >> 3) * 4 + (q & 1) * 2;
+    int2* d = reinterpret_cast<int2*>(sx + uint32_t((j >> 1) * nch + chunk) * 16u + (j & 1) * 8);
+    d[0] = make_int2(v.x, v.y);
+    d[2] = make_int2(v.z, v.w);  // the next chunk's
+  }
+  __syncthreads();
+
+  float acc[R] = {};
+  const bool f16 = p.wscale_dtype == TG_DT_F16;
+  if (live) {
+    for (int c = c0 + lane; c < c1; c += 32 * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int cc = c + 32 * u;
+        if (cc >= c1) break;
+        const uint4 a = *reinterpret_cast<const uint4*>(sx + uint32_t(cc) * 16u);
+        const uint4 b = *reinterpret_cast<const uint4*>(sx + uint32_t(nch + cc) * 16u);
+        const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint32_t v[4] = {uint32_t(w[u][r].x), uint32_t(w[u][r].y), uint32_t(w[u][r].z), uint32_t(w[u][r].w)};
+#pragma unroll
+          for (int q = 0; q < SV; ++q) {
+            int sum = 0;
+#pragma unroll
+            for (int j = q * (4 / SV); j < (q + 1) * (4 / SV); ++j) {
+              sum = __dp4a(int(v[j] & 0xf0f0f0f0u), int(x[2 * j + 1]), sum);
+              sum = __dp4a(int((v[j] << 4) & 0xf0f0f0f0u), int(x[2 * j]), sum);
+            }
+            acc[r] = fmaf(__int2float_rn(sum), sc[u][r].get(q, f16), acc[r]);
+          }
+        }
+      }
+      if (c + 32 * U < c1) load(c + 32 * U);  // the other warps' products cover it
+    }
+  }
+
+  // Sum over the warp's lanes, then over the K parts of each row group.
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float v = acc[r];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == r) partial[warp][r] = v;
+  }
+  __syncthreads();
+  const int i = threadIdx.x;
+  if (i < groups_per_cta * R) {
+    const int g = i / R, r = i - g * R;
+    const uint32_t n = (blockIdx.x * uint32_t(groups_per_cta) + uint32_t(g)) * R + uint32_t(r);
+    if (n < N) {
+      float v = 0.0f;
+      for (int k = 0; k < kp; ++k) v += partial[g * kp + k][r];
+      v = v * 0.0625f * p.xscale[0];
+      if (p.bias) v += load_as_f32(p.bias, p.bias_dtype, size_t(n));
+      store_f32_as(p.out, p.out_dtype, size_t(n), v);
+    }
   }
 }
 

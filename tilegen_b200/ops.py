@@ -390,8 +390,9 @@ def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, 
     most ``INT4_MAX_M``; ``w4 [N, K/2]`` uint8 in the layout of
     ``tilegen_b200.quant.pack_int4`` and ``wscale [N, K/group]`` fp32/fp16/bf16 as
     ``quantize_convrot_weight_int4`` returns them (``group``, read off the shapes,
-    32, 64, 128 or 256; ``K`` a multiple of 128); ``bias [N]`` or None.  A row's
-    result does not depend on the other rows.  ``out``: an optional contiguous
+    32, 64, 128 or 256; ``K`` a multiple of 128); ``bias [N]`` or None.  From
+    two rows up a row's result does not depend on the others; one row alone is added
+    up in another order (another kernel).  ``out``: an optional contiguous
     ``[M, N]`` ``out_dtype`` tensor to write into.
     """
     fn = "int4_gemv_dequant"
