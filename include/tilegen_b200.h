@@ -237,7 +237,7 @@ int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
  *   wscale  [N, K/group] of wscale_dtype (TG_DT_F32/F16/BF16), 16-B aligned
  *   group   32, 64, 128 or 256 consecutive codes; K % group == 0
  *   bias    [N] of bias_dtype or NULL; out [M, N] of out_dtype (any N)
- * M == 0 is a no-op; TG_ERR_UNSUPPORTED for M > TG_INT4_MAX_M.
+ * M == 0 is a no-op; TG_ERR_UNSUPPORTED for M > TG_INT4_MAX_M or N > 2^31 - 256.
  */
 int tg_int4_gemv_dequant(const int8_t *xq, const float *xscale, const uint8_t *w4, const void *wscale,
                          int wscale_dtype, int group, const void *bias, int bias_dtype, int64_t M, int64_t N,
@@ -290,7 +290,8 @@ size_t tg_route_experts_workspace(int64_t T, int64_t E);
  *            aligned, or NULL: with `rows` and large products the rows are
  *            gathered there first; without it (or with less) in the kernel.  It
  *            needs no initial value; calls that share it must not overlap
- * xq, wq and out 16-B aligned; E <= TG_MAX_EXPERTS.  R == 0 is a no-op.
+ * xq, wq and out 16-B aligned; E <= TG_MAX_EXPERTS; M, R and E*N at most
+ * 2^31 - 256.  R == 0 is a no-op.
  */
 int tg_int8_grouped_gemm_dequant(const int8_t *xq, const float *xscale, int64_t M, const int8_t *wq,
                                  const float *wscale, int64_t wscale_numel, const void *bias, int bias_dtype,

@@ -138,7 +138,7 @@ def _int4(xq=P, xs=P, w4=P, ws=P, wdt=1, group=128, bias=None, bdt=0, m=1, n=16,
     ({"k": 384, "group": 256}, UNS), ({"xq": None}, ARG), ({"xs": None}, ARG), ({"w4": None}, ARG), ({"ws": None}, ARG),
     ({"out": None}, ARG), ({"w4": ctypes.c_void_p(264)}, MIS), ({"xq": ctypes.c_void_p(8)}, MIS),
     ({"out": ctypes.c_void_p(257)}, MIS), ({"ws": ctypes.c_void_p(257)}, MIS), ({"m": 0, "xq": None, "out": None}, OK),
-    ({"n": 1 << 31}, UNS),
+    ({"n": 1 << 31}, UNS), ({"n": (1 << 31) - 255}, UNS), ({"n": (1 << 31) - 256, "xq": None}, ARG),
 ])
 def test_int4_entry_checks(kwargs, status):
     assert _int4(**kwargs) == status
@@ -172,7 +172,8 @@ def _grouped(xq=P, xs=P, m=4, wq=P, ws=P, wn=1, bias=None, bdt=0, rows=P, offset
     ({"n": 2, "odt": 0}, UNS), ({"e": 1025}, UNS), ({"e": 1000, "n": 1 << 22}, UNS), ({"xq": None}, ARG), ({"xs": None}, ARG), ({"wq": None}, ARG),
     ({"ws": None}, ARG), ({"offsets": None}, ARG), ({"out": None}, ARG), ({"xq": ctypes.c_void_p(8)}, MIS),
     ({"wq": ctypes.c_void_p(8)}, MIS), ({"out": ctypes.c_void_p(8)}, MIS), ({"rows": ctypes.c_void_p(2)}, MIS),
-    ({"r": 0, "out": None}, OK), ({"m": 0, "r": 0, "xq": None}, OK),
+    ({"e": 1, "n": (1 << 31) - 248}, UNS), ({"e": 2, "n": (1 << 30) - 64}, UNS), ({"r": (1 << 31) - 255, "m": 1 << 30}, UNS),
+    ({"m": (1 << 31) - 255}, UNS), ({"r": 0, "out": None}, OK), ({"m": 0, "r": 0, "xq": None}, OK),
 ])
 def test_grouped_entry_checks(kwargs, status):
     need = _lib.lib().tg_int8_grouped_gemm_dequant_workspace

@@ -19,6 +19,9 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr int64_t kRotQuantMaxK = 32768;
+// Most rows that kernels with tiles of up to 256 rows and 32-bit row numbers take:
+// the numbers of a last tile's absent rows stay below 2^31 too.
+constexpr int64_t kMaxTiledRows = (int64_t(1) << 31) - 256;
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -1226,7 +1229,7 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   if (!is_dtype(out_dtype) || !is_dtype(wscale_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
   if (group != 32 && group != 64 && group != 128 && group != 256) return TG_ERR_UNSUPPORTED;
   if (M > TG_INT4_MAX_M || K % 128 != 0 || K % group != 0) return TG_ERR_UNSUPPORTED;
-  if (N >= (int64_t(1) << 31) || K > kRotQuantMaxK) return TG_ERR_UNSUPPORTED;
+  if (N > kMaxTiledRows || K > kRotQuantMaxK) return TG_ERR_UNSUPPORTED;
   if (M == 0) return TG_OK;
   if (!xq || !xscale || !w4 || !wscale || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(w4) || !aligned16(wscale)) return TG_ERR_MISALIGNED;
@@ -1513,8 +1516,8 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
   if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
   if ((!rows && R > M) || (R > 0 && M == 0)) return TG_ERR_INVALID_ARG;
   if (K % 16 != 0 || (N * int64_t(dtype_bytes(out_dtype))) % 16 != 0) return TG_ERR_UNSUPPORTED;
-  if (E > tg::route::MAX_E || M >= (int64_t(1) << 31) || R >= (int64_t(1) << 31) || K >= (int64_t(1) << 31) ||
-      N >= (int64_t(1) << 31) || E * N >= (int64_t(1) << 31))
+  if (E > tg::route::MAX_E || M > kMaxTiledRows || R > kMaxTiledRows || K >= (int64_t(1) << 31) ||
+      N > kMaxTiledRows || E * N > kMaxTiledRows)
     return TG_ERR_UNSUPPORTED;
   if (R == 0) return TG_OK;
   if (!xq || !xscale || !wq || !wscale || !offsets || !out) return TG_ERR_INVALID_ARG;
