@@ -67,8 +67,8 @@ def test_types(cuda, out_dtype, scale_dtype, bias_dtype):
         _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, out_dtype), xq, xs, codes, ws, bias)
 
 
-@pytest.mark.parametrize("n,k,group", [(1, 128, 32), (1, 128, 128), (15, 128, 64), (16, 256, 256), (17, 1408, 128), (33, 14080, 128),
-                                       (1001, 5120, 32), (5120, 13824, 256), (13823, 5120, 128)])
+@pytest.mark.parametrize("n,k,group", [(1, 128, 32), (1, 128, 128), (15, 128, 64), (16, 256, 256), (17, 1408, 128),
+                                       (33, 14080, 128), (2000, 32768, 32), (70000, 256, 64), (1001, 5120, 32), (5120, 13824, 256), (13823, 5120, 128)])
 def test_odd_and_block_shapes(cuda, n, k, group):
     for m in (1, 2, 4, 5, 40):
         xq, xs, codes, ws, bias = _case(m, n, k, group, torch.bfloat16, torch.float16, seed=n + k + m)

@@ -1133,11 +1133,10 @@ int gemv4_parts(int64_t N, int64_t K, int sms) {
 }
 
 template <int U, int SV, bool S4>
-int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, int dev, cudaStream_t st) {
-  static uint32_t attr_done[kMaxDevices];
-  auto kern = tg::gemv_i4_one_kernel<U, SV, S4>;
-  if (!ensure_smem_attr(kern, dev, uint32_t(kRotQuantMaxK), attr_done)) return TG_ERR_CUDA;
-  return launch_dependent(kern, p, dim3(unsigned(ctas)), tg::gemv4one::THREADS, uint32_t(p.K), st);
+int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, cudaStream_t st) {
+  static_assert(kRotQuantMaxK <= 48 * 1024 - 256, "a row fits the shared memory of any launch");
+  return launch_dependent(tg::gemv_i4_one_kernel<U, SV, S4>, p, dim3(unsigned(ctas)), tg::gemv4one::THREADS,
+                          uint32_t(p.K), st);
 }
 
 // Two chunks of a row under way at once need registers that leave three CTAs per
@@ -1147,22 +1146,22 @@ int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, int dev, cuda
 // (480 CTAs) 11.4 / 8.3, 2048 x 1536 (two chunks a lane) 2.35 / 2.15.  Groups of 32
 // with fp32 scales are 16 more registers a chunk, too many: 12.7 / 11.2.
 template <int SV, bool S4>
-int launch_gemv4_one_sv(const tg::GemvI4OneParams& p, int sms, int dev, cudaStream_t st) {
+int launch_gemv4_one_sv(const tg::GemvI4OneParams& p, int sms, cudaStream_t st) {
   using namespace tg::gemv4one;
   const int64_t row_groups = (int64_t(p.N) + R - 1) / R, per_cta = WARPS / p.kp;
   const int64_t ctas = (row_groups + per_cta - 1) / per_cta;
   if constexpr (SV < 4 || !S4) {
-    if (ctas <= 3 * int64_t(sms) && p.part_chunks > 64) return launch_gemv4_one_t<2, SV, S4>(p, ctas, dev, st);
+    if (ctas <= 3 * int64_t(sms) && p.part_chunks > 64) return launch_gemv4_one_t<2, SV, S4>(p, ctas, st);
   }
-  return launch_gemv4_one_t<1, SV, S4>(p, ctas, dev, st);
+  return launch_gemv4_one_t<1, SV, S4>(p, ctas, st);
 }
 
-int launch_gemv4_one(const tg::GemvI4OneParams& p, int sv, int sms, int dev, cudaStream_t st) {
+int launch_gemv4_one(const tg::GemvI4OneParams& p, int sv, int sms, cudaStream_t st) {
   const bool s4 = p.wscale_dtype == TG_DT_F32;
   switch (sv) {
-    case 4: return s4 ? launch_gemv4_one_sv<4, true>(p, sms, dev, st) : launch_gemv4_one_sv<4, false>(p, sms, dev, st);
-    case 2: return s4 ? launch_gemv4_one_sv<2, true>(p, sms, dev, st) : launch_gemv4_one_sv<2, false>(p, sms, dev, st);
-    default: return s4 ? launch_gemv4_one_sv<1, true>(p, sms, dev, st) : launch_gemv4_one_sv<1, false>(p, sms, dev, st);
+    case 4: return s4 ? launch_gemv4_one_sv<4, true>(p, sms, st) : launch_gemv4_one_sv<4, false>(p, sms, st);
+    case 2: return s4 ? launch_gemv4_one_sv<2, true>(p, sms, st) : launch_gemv4_one_sv<2, false>(p, sms, st);
+    default: return s4 ? launch_gemv4_one_sv<1, true>(p, sms, st) : launch_gemv4_one_sv<1, false>(p, sms, st);
   }
 }
 
@@ -1272,7 +1271,7 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
     q.part_chunks = int((K / 32 + q.kp - 1) / q.kp);
     q.prefetch = N * K / 2 <= kGemvPrefetchMaxBytes ? 1 : 0;
     q.out = out;
-    return launch_gemv4_one(q, sv, info.sms_all, dev, st);
+    return launch_gemv4_one(q, sv, info.sms_all, st);
   }
   // 16-row tiles an SM gets.  Where they are few, a CTA's steps are what takes the
   // time, and two blocks a step halve them; where they are many, one block a step

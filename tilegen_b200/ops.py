@@ -382,7 +382,8 @@ _F32, _I8, _U8, _I32 = (torch.float32,), (torch.int8,), (torch.uint8,), (torch.i
 
 
 def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor,
-                      bias: torch.Tensor | None, out_dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
+                      bias: torch.Tensor | None, out_dtype: torch.dtype,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Few rows of int8 codes times a 4-bit weight with group scales (``tg_int4_gemv_dequant``):
     ``out[m, n] = (sum_g wscale[n, g] * (xq[m, g] . w4[n, g])) * xscale[m] + bias[n]``.
 

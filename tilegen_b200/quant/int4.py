@@ -71,7 +71,8 @@ def quantize_convrot_weight_int4(weight: torch.Tensor, group_size: int = 256, sc
 
 
 def int4_linear(x: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor, bias: torch.Tensor | None = None,
-                out_dtype: torch.dtype | None = None, group_size: int = 256, input_act: str | None = None) -> torch.Tensor:
+                out_dtype: torch.dtype | None = None, group_size: int = 256,
+                input_act: str | None = None) -> torch.Tensor:
     """``input_act(x)`` rotated and quantised row-wise, times a 4-bit weight.
 
     ``x [..., K]`` fp16/bf16 on a CUDA device; ``group_size`` and ``input_act`` as
@@ -88,6 +89,8 @@ def int4_linear(x: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor, bias: t
     m, n = xq.shape[0], w4.shape[0]
     if m <= ops.INT4_MAX_M:
         return ops.int4_gemv_dequant(xq, xscale, w4, wscale, bias, out_dtype).reshape(*x.shape[:-1], n)
-    blocks = [ops.int4_gemv_dequant(xq[s:s + ops.INT4_MAX_M], xscale[s:s + ops.INT4_MAX_M], w4, wscale, bias, out_dtype)
-              for s in range(0, m, ops.INT4_MAX_M)]
-    return torch.cat(blocks).reshape(*x.shape[:-1], n)
+    y = torch.empty(m, n, dtype=out_dtype, device=x.device)
+    for s in range(0, m, ops.INT4_MAX_M):
+        e = s + ops.INT4_MAX_M
+        ops.int4_gemv_dequant(xq[s:e], xscale[s:e], w4, wscale, bias, out_dtype, out=y[s:e])
+    return y.reshape(*x.shape[:-1], n)
