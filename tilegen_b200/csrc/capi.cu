@@ -1142,9 +1142,9 @@ int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, cudaStream_t 
 // Two chunks of a row under way at once need registers that leave three CTAs per
 // SM, and help where the launch is one wave of those and a lane has more than two
 // chunks; otherwise four CTAs per SM with one chunk each carry more.  Measured (K x
-// N, two / one, us): 13824 x 5120 8.6 / 10.1, 5120 x 5120 5.2 / 5.7; 5120 x 15360
-// (480 CTAs) 11.4 / 8.3, 2048 x 1536 (two chunks a lane) 2.35 / 2.15.  Groups of 32
-// with fp32 scales are 16 more registers a chunk, too many: 12.7 / 11.2.
+// N, two / one, us): 13824 x 5120 8.6 / 9.6, 5120 x 5120 5.2 / 5.35; 5120 x 15360
+// (480 CTAs) 11.4 / 8.0, 2048 x 1536 (two chunks a lane) 2.3 / 2.15.  Groups of 32
+// with fp32 scales are 16 more registers a chunk and spilled: 12.7 / 11.2.
 template <int SV, bool S4>
 int launch_gemv4_one_sv(const tg::GemvI4OneParams& p, int sms, cudaStream_t st) {
   using namespace tg::gemv4one;
@@ -1275,9 +1275,9 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   }
   // 16-row tiles an SM gets.  Where they are few, a CTA's steps are what takes the
   // time, and two blocks a step halve them; where they are many, one block a step
-  // leaves room for the rings of more CTAs.  Measured (two blocks / one, us): 4 rows,
-  // K x N = 5120 x 5120 6.1 / 6.7, 13824 x 5120 13.5 / 13.4; 5120 x 15360 with 8
-  // rows 13.3 / 9.7, with 16 rows 14.0 / 12.1.
+  // leaves room for the rings of more CTAs.  Measured (K x N, two blocks / one, us):
+  // 8 rows, 5120 x 5120 5.3 / 6.5, 13824 x 5120 11.3 / 12.5, 5120 x 15360 12.6 / 8.8;
+  // 16 rows, 5120 x 5120 6.2 / 8.7, 13824 x 5120 12.0 / 18.5, 5120 x 15360 13.5 / 10.4.
   const int64_t tiles = (N + 15) / 16, sms = info.sms_all;
   const int want = int(std::max<int64_t>(1, std::min<int64_t>(8, (tiles + sms - 1) / sms)));
   const bool few = want <= 3;

@@ -48,10 +48,11 @@
 // CTA first lays the row out in shared memory as [half][chunk][16 bytes], two
 // 128-bit reads a chunk that serve the four rows.  K x N, this form / the ring (us):
 // 2048 x 1536 2.2 / 2.9, 5120 x 15360 8.3 / 9.4, 5120 x 5120 5.3 / 5.3, 13824 x 5120
-// 8.6 / 11.5.  It is bound by the weight's latency (one wave of loads that depend on
-// the CTAs resident).  Written for more rows it took, with two rows, 13.1 us on
-// 5120 x 15360 and 11.8 on 13824 x 5120 (the ring 9.7 and 13.6), and with four 16.3
-// and 20.7 (the ring as with two).
+// 8.6 / 11.5.  It is bound by the loads' latency: the launch is about one wave, and
+// what it reads per us depends on the loads its resident warps have under way.
+// Written for more rows it took, with two rows, 13.1 us on 5120 x 15360 and 11.8 on
+// 13824 x 5120 (the ring 8.9 and 11.4), and with four 16.3 and 20.7 (the ring as
+// with two).
 #pragma once
 
 #include "common.cuh"
