@@ -62,6 +62,35 @@ def test_weight_quantiser_error(scale_group, scale_dtype):
     assert (got[3] == 0).all()
 
 
+@pytest.mark.parametrize("scale_dtype,spread", [(dt, s) for dt in (torch.float32, torch.bfloat16) for s in (1e-4, 1e-6, 1e-9, 1e-30)]
+                         + [(torch.float16, s) for s in (1e-4, 1e-5, 1e-6)])
+def test_weight_quantiser_keeps_small_weights(scale_dtype, spread):
+    """A value is off by at most half the step, and the step is the group's absmax/7 up to the division's rounding
+    and its own (fp16 below 2^-14: up by less than 2^-24, with no code clipped)."""
+    w = torch.randn(16, 512, generator=torch.Generator().manual_seed(5)) * spread
+    w[2] = 0
+    w4, ws = quantize_convrot_weight_int4(w, 1, 64, scale_dtype)
+    got = unpack_int4(w4).double().view(16, 8, 64) * ws.double()[..., None]
+    exact = w.double().view(16, 8, 64)
+    half = torch.finfo(scale_dtype).eps / 2
+    step = exact.abs().amax(-1, keepdim=True) / 7 * (1 + 2.0 ** -24) * (1 + half) + (2.0 ** -24 if scale_dtype == torch.float16 else 0)
+    assert ((got - exact).abs() <= step / 2 + 7 * step * half + 2.0 ** -149).all()
+    assert (got[2] == 0).all()
+
+
+def test_weight_quantiser_fp16_scales_at_the_lower_end():
+    w = torch.randn(4, 256, generator=torch.Generator().manual_seed(6))
+    with pytest.raises(ValueError, match="too small"):
+        quantize_convrot_weight_int4(w * 1e-9)
+    quantize_convrot_weight_int4(w * 1e-9, scale_dtype=torch.bfloat16)
+    w4, ws = quantize_convrot_weight_int4(torch.zeros(4, 256))
+    assert (unpack_int4(w4) == 0).all() and (ws > 0).all()
+    assert quantize_convrot_weight_int4(torch.zeros(0, 256))[1].shape == (0, 2)
+    w[1] *= 1e-12  # one small row among others is not a reason to refuse: its values are below 2^-25
+    w4, ws = quantize_convrot_weight_int4(w, 1)
+    assert ((unpack_int4(w4).double().view(4, 2, 128)[1] * ws.double()[1, :, None]).abs() <= 2.0 ** -24).all()
+
+
 def test_weight_quantiser_refusals():
     w = torch.zeros(4, 256)
     for kwargs in ({"scale_group": 16}, {"scale_group": 512}, {"scale_dtype": torch.float64}, {"group_size": 512}):

@@ -16,6 +16,7 @@ from .. import ops
 from ..kernels.hadamard import build_hadamard, rotate_by_group
 
 _CODE_MAX = 7  # symmetric codes: -7..7 (the kernel also reads -8)
+_F16_STEP = 2.0 ** -24  # between fp16's subnormal numbers, and the smallest of them
 
 
 def pack_int4(codes: torch.Tensor) -> torch.Tensor:
@@ -47,7 +48,11 @@ def quantize_convrot_weight_int4(weight: torch.Tensor, group_size: int = 256, sc
 
     ``group_size`` is the rotation's (``1``: none), ``scale_group`` the channels that
     share a scale.  A scale is absmax/7 in fp32, rounded to ``scale_dtype``; the codes
-    divide by the rounded one.  Done once per weight, in fp32, on the weight's device.
+    divide by the rounded one.  fp32 and bf16 scales are at least 2^-126.  fp16 scales
+    below 2^-14 are rounded up to a multiple of 2^-24, so that no code is clipped; where
+    other groups are larger, values up to 2^-25 of a group thus become 0, and a weight
+    none of whose values reaches 7 * 2^-24 is refused (fp32 and bf16 scales hold it).
+    Done once per weight, in fp32, on the weight's device.
     """
     if weight.ndim != 2:
         raise ValueError(f"weight must be 2D [N,K], got {tuple(weight.shape)}")
@@ -62,8 +67,16 @@ def quantize_convrot_weight_int4(weight: torch.Tensor, group_size: int = 256, sc
     if group_size != 1:
         w = rotate_by_group(w, build_hadamard(group_size, w.device, w.dtype), group_size)
     w = w.view(n, k // scale_group, scale_group)
-    # The smallest scale that every scale_dtype holds as a normal number.
-    scale = (w.abs().amax(dim=-1) / _CODE_MAX).clamp_min(2.0 ** -14).to(scale_dtype)
+    scale = w.abs().amax(dim=-1) / _CODE_MAX
+    if scale_dtype == torch.float16:
+        most = scale.amax() if scale.numel() else scale.new_zeros(())
+        if bool((most > 0) & (most < _F16_STEP)):
+            raise ValueError("the weight is too small for fp16 scales: use fp32 or bf16 ones")
+        scale = torch.where(scale < torch.finfo(torch.float16).tiny, torch.ceil(scale / _F16_STEP) * _F16_STEP, scale)
+        scale = scale.clamp_min(_F16_STEP)
+    else:
+        scale = scale.clamp_min(torch.finfo(scale_dtype).tiny)
+    scale = scale.to(scale_dtype)
     if not bool(torch.isfinite(scale).all()):
         raise ValueError(f"the weight has values that a {scale_dtype} scale cannot hold")
     codes = torch.round(w / scale.float()[..., None]).clamp_(-_CODE_MAX, _CODE_MAX).to(torch.int8)
