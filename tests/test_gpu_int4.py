@@ -75,6 +75,26 @@ def test_odd_and_block_shapes(cuda, n, k, group):
         _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, torch.bfloat16), xq, xs, codes, ws, bias)
 
 
+@pytest.mark.parametrize("m", [9, 12, 16])
+def test_wide_weight_of_the_longest_rows_and_finest_scales(cuda, m):
+    """Where 64 rows' scales do not fit an SM's shared memory (fp32 scales of 32 codes, K past 22000)."""
+    for k in (22656, 22784, 32768):
+        xq, xs, codes, ws, bias = _case(m, 7131, k, 32, torch.float32, torch.float32, seed=m)
+        w4 = pack_int4(codes)
+        y = ops.int4_gemv_dequant(xq, xs, w4, ws, bias, torch.float32)
+        _check(y, xq, xs, codes, ws, bias)
+        # the same rows in the other forms: a row's bits depend neither on M nor on the tile
+        assert torch.equal(ops.int4_gemv_dequant(xq[:4], xs[:4], w4, ws, bias, torch.float32), y[:4])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_wide_weight_of_nine_to_sixteen_rows(cuda, scale_dtype, group):
+    for m in (9, 14, 16):
+        xq, xs, codes, ws, bias = _case(m, 7300, 1280, group, scale_dtype, torch.float16, seed=m)
+        _check(ops.int4_gemv_dequant(xq, xs, pack_int4(codes), ws, bias, torch.float32), xq, xs, codes, ws, bias)
+
+
 def test_extreme_codes_do_not_overflow(cuda):
     """-128 times -8 over the largest K the group allows: the int32 sums and 16-fold codes hold them."""
     k = 32768

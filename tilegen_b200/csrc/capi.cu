@@ -1115,12 +1115,24 @@ bool make_tmap_blocks(CUtensorMap* m, const void* base, uint64_t row_bytes, uint
 
 // Shared memory of a launch with `stages` ring slots: the ring (or the partial
 // tiles) and the scales.
-uint32_t gemv4_smem(int m, int mt, int rows, int kb, int groups, bool s4, int stages) {
+constexpr uint32_t gemv4_smem(int m, int mt, int rows, int kb, int groups, bool s4, int stages) {
   using namespace tg::gemv4;
   const uint32_t ring = uint32_t(stages) * (w_bytes(kb, rows) + x_bytes(kb, m));
   return std::max(ring + scale_bytes(rows, groups, s4), uint32_t(WK * 8 * mt * rows) * 4u) +
          1024u + uint32_t(8 * mt - m) * 128u;  // alignment, and the rows past m that are read and dropped
 }
+
+constexpr uint32_t kGemv4Static = 512;  // barriers and the abort flag, rounded up
+
+// The form with 32 weight rows a CTA fits an SM at every documented size: two ring
+// slots beside the scales of the longest rows in the finest groups (and the dropped
+// rows of any m, which need less of the ring).  64 or 96 rows' scales may not.
+constexpr bool gemv4_always_fits(int mt, int kb) {
+  return gemv4_smem(8 * mt, mt, 32, kb, int(kRotQuantMaxK / 32), true, 2) + 8u * uint32_t(mt) * 128u + kGemv4Static +
+             1024u <= kSmemPerSm;
+}
+static_assert(gemv4_always_fits(1, 1) && gemv4_always_fits(1, 2) && gemv4_always_fits(2, 2) &&
+              gemv4_always_fits(4, 1) && gemv4_always_fits(8, 1), "a form for every size");
 
 // K parts per group of four weight rows, as gemv_parts: the fewest that put two
 // CTAs on every SM, each part keeping two chunks a lane.
@@ -1170,14 +1182,13 @@ template <int MT, int RT, int WR, int KB, int SV, bool S4>
 int launch_gemv4_t(const int8_t* xq, const uint8_t* w4, tg::GemvI4Params p, int want, int dev, cudaStream_t st) {
   using namespace tg::gemv4;
   static uint32_t attr_done[kMaxDevices];
-  constexpr uint32_t kStatic = 512;  // barriers and the abort flag, rounded up
   auto kern = tg::gemv_i4_kernel<MT, RT, WR, KB, SV, S4>;
-  if (!ensure_smem_attr(kern, dev, kSmemPerCtaMax - kStatic, attr_done)) return TG_ERR_CUDA;
+  if (!ensure_smem_attr(kern, dev, kSmemPerCtaMax - kGemv4Static, attr_done)) return TG_ERR_CUDA;
   constexpr int kRows = rows(RT, WR);
   const int steps = (p.K / 128 + KB * WK - 1) / (KB * WK);
   int stages = std::min(MAX_STAGES, std::max(2, steps));
   auto fits = [&](int s, int ctas) {
-    return uint64_t(ctas) * (gemv4_smem(p.M, MT, kRows, KB, p.groups, S4, s) + kStatic + 1024u) <= kSmemPerSm;
+    return uint64_t(ctas) * (gemv4_smem(p.M, MT, kRows, KB, p.groups, S4, s) + kGemv4Static + 1024u) <= kSmemPerSm;
   };
   while (want > 1 && !fits(std::min(3, stages), want)) --want;
   while (stages > 2 && !fits(stages, want)) --stages;
@@ -1283,15 +1294,19 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
   const bool few = want <= 3;
   if (M <= 8) return few ? launch_gemv4<1, 2, 1, 2>(xq, w4, p, sv, (want + 1) / 2, dev, st)
                          : launch_gemv4<1, 2, 1, 1>(xq, w4, p, sv, (want + 1) / 2, dev, st);
-  if (M <= 16) return few ? launch_gemv4<2, 1, 2, 2>(xq, w4, p, sv, (want + 1) / 2, dev, st)
-                          : launch_gemv4<2, 2, 2, 1>(xq, w4, p, sv, 2, dev, st);
+  if (M <= 16) {
+    const int rc = few ? launch_gemv4<2, 1, 2, 2>(xq, w4, p, sv, (want + 1) / 2, dev, st)
+                       : launch_gemv4<2, 2, 2, 1>(xq, w4, p, sv, 2, dev, st);
+    // Very long rows of fine fp32 scales leave no room for 64 rows of them.
+    return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<2, 1, 2, 2>(xq, w4, p, sv, 1, dev, st) : rc;
+  }
   if (M <= 32) return launch_gemv4<4, 2, 1, 1>(xq, w4, p, sv, std::min(2, (want + 1) / 2), dev, st);
   // 64 or 96 rows a CTA, one CTA per SM: whichever takes the fewer rows of them in all.
   const int64_t t32 = (N + 31) / 32;
   const int64_t cost2 = (t32 + 2 * sms - 1) / (2 * sms) * 2, cost3 = (t32 + 3 * sms - 1) / (3 * sms) * 3;
   const int rc = cost3 < cost2 ? launch_gemv4<8, 2, 3, 1>(xq, w4, p, sv, 1, dev, st)
                                : launch_gemv4<8, 2, 2, 1>(xq, w4, p, sv, 1, dev, st);
-  // Very long rows of fine scales leave no room for so many rows of them.
+  // As above.
   return rc == TG_ERR_UNSUPPORTED ? launch_gemv4<8, 2, 1, 1>(xq, w4, p, sv, 2, dev, st) : rc;
 }
 
