@@ -116,6 +116,18 @@ def test_expert_weights_are_each_experts_weight():
         quantize_convrot_expert_weights(w[0])
 
 
+@pytest.mark.parametrize("package", ["kernels", "quant", "runtime", "comfyui"])
+def test_every_module_has_its_alias(package):
+    """``tilegen.<package>.<module>`` is the ``tilegen_b200`` module, for every module file there is."""
+    import importlib
+    import pkgutil
+
+    mine = importlib.import_module("tilegen_b200." + package)
+    for info in pkgutil.iter_modules(mine.__path__):
+        name = f"{package}.{info.name}"
+        assert importlib.import_module("tilegen." + name) is importlib.import_module("tilegen_b200." + name)
+
+
 # ---------------------------------------------------------------- Python refusals
 def test_cpu_tensors_are_refused():
     i8, f = torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2)

@@ -3,7 +3,8 @@
 Every module of the reference package's public surface is registered under its
 reference name, so ``from tilegen.kernels.int8_convrot import _eager_quantize``
 and friends return the very same objects as the ``tilegen_b200`` modules (patching
-one patches the other).
+one patches the other).  The modules of these packages that the reference does not
+have (``quant.int4``, ``quant.experts``) are registered likewise.
 """
 import importlib
 import sys
@@ -11,6 +12,7 @@ import sys
 _MODULES = (
     "kernels", "kernels.hadamard", "kernels.int8_convrot",
     "quant", "quant.weight", "quant.int8_ops", "quant.rowwise",
+    "quant.int4", "quant.experts",
     "runtime", "runtime.device", "runtime.nvrtc",
     "comfyui", "comfyui.backend", "comfyui.nodes",
 )
