@@ -332,6 +332,19 @@ def test_grouped_strides_and_refusals(cuda):
     assert ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, None, offsets, f16, rows=rows[:0]).shape == (0, 64)
 
 
+def test_grouped_scale_shapes(cuda):
+    """[E, N] scales by any of their unambiguous shapes; a transposed one, of as many elements, is refused."""
+    xq, xs, wq, ws, bias, offsets, rows = _group_case([3, 4], 64, 128, 20, torch.float32, seed=2)
+    y = ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, bias, offsets, torch.float16, rows=rows)
+    for same in (ws[..., None], ws.reshape(-1), ws.t().contiguous().t()):
+        assert torch.equal(ops.int8_grouped_gemm_dequant(xq, xs, wq, same, bias, offsets, torch.float16, rows=rows), y)
+    a = ops.int8_grouped_gemm_dequant(xq, xs, wq, ws[:, 0], bias, offsets, torch.float16, rows=rows)
+    assert torch.equal(ops.int8_grouped_gemm_dequant(xq, xs, wq, ws[:, :1], bias, offsets, torch.float16, rows=rows), a)
+    for bad in (ws.t(), ws.t().contiguous(), ws[0]):
+        with pytest.raises(ValueError, match="wscale"):
+            ops.int8_grouped_gemm_dequant(xq, xs, wq, bad, bias, offsets, torch.float16, rows=rows)
+
+
 # ---------------------------------------------------------------- combine
 def _check_combine(y, place, weights, residual, out=None):
     got = ops.combine_experts(y, place, weights, residual=None if residual is None else residual.clone(), out=out)

@@ -142,6 +142,22 @@ def test_cpu_tensors_are_refused():
         ops.combine_experts(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
 
 
+@pytest.mark.parametrize("e,n", [(3, 8), (1, 16), (2, 4)])
+def test_expert_scale_shapes(e, n):
+    """A wscale of the right number of elements in the wrong order is refused."""
+    cpu = torch.device("cpu")
+    for shape in ((), (1,), (1, 1), (e,), (e, 1), (e, n), (e, n, 1), (e, 1, n), (e * n,)):
+        ops._expert_scales("f", torch.zeros(shape), e, n, cpu)
+    for bad in ((n,), (e + 1,), (e, n - 1), (2, e, n), (0,), (e, 0)) + (((n, e), (n, 1, e)) if e > 1 else ()):
+        if (e == 1 and bad == (n,)):
+            continue  # one expert's scales
+        with pytest.raises(ValueError, match="wscale"):
+            ops._expert_scales("f", torch.zeros(bad), e, n, cpu)
+    for bad in (torch.zeros(e, n).double(), [1.0], torch.zeros(e, n, device="meta")):
+        with pytest.raises(ValueError, match="wscale"):
+            ops._expert_scales("f", bad, e, n, cpu)
+
+
 def test_layer_functions_check_shapes():
     with pytest.raises(ValueError, match="differ"):
         int4_linear(torch.zeros(2, 256), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 1))

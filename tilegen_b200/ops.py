@@ -481,6 +481,17 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
     return ExpertRoutes(weights, ids, offsets, rows, place)
 
 
+def _expert_scales(fn: str, t, e: int, n: int, dev: torch.device) -> None:
+    """``t``: one fp32 scale on ``dev``, or ``[e]``, ``[e, n]`` or ``[e * n]`` of them (dimensions of one aside),
+    or ValueError: a transposed one has as many elements."""
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.float32:
+        raise ValueError(f"{fn}: wscale must be fp32 on {dev}")
+    shape = tuple(t.shape)
+    if shape != (e, n) and [d for d in shape if d != 1] not in ([], [d for d in (e, n) if d != 1],
+                                                                [d for d in (e,) if d != 1], [e * n]):
+        raise ValueError(f"{fn}: wscale is {shape}, expected one scale, {(e,)} or {(e, n)}")
+
+
 def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor,
                               bias: torch.Tensor | None, offsets: torch.Tensor, out_dtype: torch.dtype,
                               rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -516,9 +527,7 @@ def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.
         raise ValueError(f"{fn}: offsets has {offsets.shape[0]} elements, expected {e + 1}")
     if xscale.shape[0] != m:
         raise ValueError(f"{fn}: xscale has {xscale.shape[0]} elements, expected {m}")
-    if not isinstance(wscale, torch.Tensor) or wscale.device != dev or wscale.dtype != torch.float32 \
-            or wscale.numel() not in (1, e, e * n):
-        raise ValueError(f"{fn}: wscale must be fp32 on {dev} with 1, {e} or {e} x {n} elements")
+    _expert_scales(fn, wscale, e, n, dev)
     b_ptr, b_code = None, _lib.TG_DT_F32
     if bias is not None:
         _on(fn, "bias", bias, dev, _FLOATS, 2)
