@@ -215,6 +215,28 @@ def test_linear_against_the_rotated_product(cuda, m):
     _check(y[0], xq, xs, unpack_int4(w4), ws, bias)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_rows_do_not_depend_on_their_number(cuda, dtype):
+    k, n = 512, 77
+    w4, ws = quantize_convrot_weight_int4(torch.randn(n, k, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda))
+    x = torch.randn(130, k, device=cuda).half()
+    y = int4_linear(x, w4, ws, out_dtype=dtype)
+    for m in (2, 64, 65, 66, 128, 129):
+        assert torch.equal(int4_linear(x[:m], w4, ws, out_dtype=dtype), y[:m])
+
+
+def test_out_at_any_address(cuda):
+    """An out that starts at an odd element, for one row and for several."""
+    for m in (1, 7, 40):
+        xq, xs, codes, ws, _ = _case(m, 33, 256, 64, seed=7)
+        w4 = pack_int4(codes)
+        for dtype in (torch.float16, torch.float32):
+            out = torch.full((m * 33 + 2,), 5.0, dtype=dtype, device=cuda)
+            y = ops.int4_gemv_dequant(xq, xs, w4, ws, None, dtype, out=out[1:-1].view(m, 33))
+            assert torch.equal(y, ops.int4_gemv_dequant(xq, xs, w4, ws, None, dtype))
+            assert out[0] == 5 and out[-1] == 5
+
+
 def test_linear_empty_and_refusals(cuda):
     w4, ws = quantize_convrot_weight_int4(torch.randn(64, 256, device=cuda))
     x = torch.randn(3, 256, device=cuda).half()

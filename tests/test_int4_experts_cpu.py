@@ -169,6 +169,25 @@ def test_layer_functions_check_shapes():
         int8_expert_ffn(torch.zeros(3, 256), torch.zeros(3, 2), up, up, 1)
 
 
+@pytest.mark.parametrize("m", [1, 2, 63, 64, 65, 66, 127, 128, 129, 130, 193, 1025])
+def test_linear_leaves_no_single_row_behind(monkeypatch, m):
+    """The blocks cover every row once, and only a one-row input goes to the one-row kernel, which adds in an order
+    of its own."""
+    seen = []
+
+    def product(xq, xs, w4, ws, bias, out_dtype, out=None):
+        assert 1 <= xq.shape[0] <= ops.INT4_MAX_M and xs.shape[0] == xq.shape[0]
+        seen.extend(xq[:, 0].tolist())
+        assert xq.shape[0] > 1 or m == 1
+        return torch.zeros(xq.shape[0], 5) if out is None else out.zero_()
+
+    monkeypatch.setattr(ops, "quantize_act", lambda x, g, a: (x, x[:, 0]))
+    monkeypatch.setattr(ops, "int4_gemv_dequant", product)
+    x = torch.arange(m, dtype=torch.float32)[:, None].repeat(1, 128)
+    assert int4_linear(x, torch.zeros(5, 64, dtype=torch.uint8), torch.zeros(5, 1)).shape == (m, 5)
+    assert seen == list(range(m))
+
+
 def test_custom_ops_trace_on_meta():
     m = torch.device("meta")
     y = torch.ops.tilegen.int4_gemv_dequant(torch.empty(3, 256, dtype=torch.int8, device=m), torch.empty(3, device=m),

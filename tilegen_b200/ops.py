@@ -426,7 +426,7 @@ def int4_gemv_dequant(xq: torch.Tensor, xscale: torch.Tensor, w4: torch.Tensor, 
         b_ptr, b_code = bias.data_ptr(), _DTYPE_CODE[bias.dtype]
     no_gradient(fn, xscale, wscale, bias)
     xq, w4, xscale, wscale = _aligned(xq), _aligned(w4), xscale.contiguous(), _aligned(wscale)
-    out = _out(fn, out, (m, n), out_dtype, dev)
+    out = _out(fn, out, (m, n), out_dtype, dev, out_dtype.itemsize)
     if m:
         _call("tg_int4_gemv_dequant", dev, xq.data_ptr(), xscale.data_ptr(), w4.data_ptr(), wscale.data_ptr(),
               _DTYPE_CODE[wscale.dtype], k // groups, b_ptr, b_code, m, n, k, _DTYPE_CODE[out_dtype], out.data_ptr())

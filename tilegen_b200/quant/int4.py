@@ -91,7 +91,8 @@ def int4_linear(x: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor, bias: t
     ``x [..., K]`` fp16/bf16 on a CUDA device; ``group_size`` and ``input_act`` as
     ``ops.quantize_act`` takes them (the rotation must be the weight's).  More rows
     than ``ops.INT4_MAX_M`` go through in blocks of that many, each of which streams
-    the weight again: for long prompts an int8 weight is the faster form.
+    the weight again: for long prompts an int8 weight is the faster form.  From two
+    rows up a row's result depends neither on the others nor on how many there are.
     """
     k = x.shape[-1]
     if k != w4.shape[-1] * 2:
@@ -103,7 +104,11 @@ def int4_linear(x: torch.Tensor, w4: torch.Tensor, wscale: torch.Tensor, bias: t
     if m <= ops.INT4_MAX_M:
         return ops.int4_gemv_dequant(xq, xscale, w4, wscale, bias, out_dtype).reshape(*x.shape[:-1], n)
     y = torch.empty(m, n, dtype=out_dtype, device=x.device)
-    for s in range(0, m, ops.INT4_MAX_M):
-        e = s + ops.INT4_MAX_M
+    s = 0
+    while s < m:
+        e = min(s + ops.INT4_MAX_M, m)
+        if m - e == 1:  # a last row alone would be added up in another order: it takes one along
+            e -= 1
         ops.int4_gemv_dequant(xq[s:e], xscale[s:e], w4, wscale, bias, out_dtype, out=y[s:e])
+        s = e
     return y.reshape(*x.shape[:-1], n)
