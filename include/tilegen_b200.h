@@ -268,7 +268,7 @@ int tg_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int to
                      float *weights, int32_t *ids, int32_t *offsets, int32_t *rows, int32_t *place, void *workspace,
                      size_t workspace_bytes, void *stream);
 
-/* Workspace bytes of tg_route_experts (0 up to 256 tokens: then NULL will do). */
+/* Workspace bytes of tg_route_experts (0 up to 256 tokens: then NULL will do; 0 for sizes that it refuses). */
 size_t tg_route_experts_workspace(int64_t T, int64_t E);
 
 /*
@@ -299,7 +299,7 @@ int tg_int8_grouped_gemm_dequant(const int8_t *xq, const float *xscale, int64_t 
                                  int64_t K, int out_dtype, void *out, void *workspace, size_t workspace_bytes,
                                  void *stream);
 
-/* Workspace bytes tg_int8_grouped_gemm_dequant makes use of when `rows` is given (0: none). */
+/* Workspace bytes tg_int8_grouped_gemm_dequant makes use of when `rows` is given (0: none, or sizes that it refuses). */
 size_t tg_int8_grouped_gemm_dequant_workspace(int64_t R, int64_t E, int64_t N, int64_t K);
 
 /*

@@ -258,6 +258,35 @@ def test_grouped_entry_checks(kwargs, status):
     assert _grouped(**kwargs) == status
 
 
+def test_workspace_sizes_of_refused_calls():
+    """Any 64-bit sizes: an answer, not the end of the process (in a child, which one division by zero would end)."""
+    import subprocess
+    import sys
+
+    code = """
+from tilegen_b200 import _lib
+L, top = _lib.lib(), 2 ** 63 - 1
+for t in (2 ** 30 + 1, 2 ** 40, 2 ** 62, top, -1, -top - 1):
+    for e in (1, 1024, 1025, top, 0, -5):
+        assert L.tg_route_experts_workspace(t, e) == 0, (t, e)
+assert 0 < L.tg_route_experts_workspace(2 ** 30, 1024) <= 256 * 32 * 1024 * 4
+sizes = (1, 2 ** 31, 2 ** 40, top, 0, -1)
+for r in sizes:
+    for e in sizes:
+        for n in sizes:
+            for k in sizes:
+                assert L.tg_int8_grouped_gemm_dequant_workspace(r, e, n, k) == 0, (r, e, n, k)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert done.returncode == 0, f"{done.returncode}: {done.stderr[-400:]}"
+
+
+@pytest.mark.parametrize("kwargs", [{"e": 1 << 62, "n": 4}, {"e": 1 << 40, "n": 1 << 40}, {"n": (1 << 63) - 8}, {"r": 1 << 62},
+                                    {"k": 1 << 62}, {"m": 1 << 62}])
+def test_grouped_sizes_past_every_limit(kwargs):
+    assert _grouped(**kwargs) == UNS
+
+
 def _combine(y=P, dt=1, r=8, place=P, w=P, t=4, k=2, res=None, n=64, out=P):
     return _lib.lib().tg_combine_experts(y, dt, r, place, w, t, k, res, n, out, None)
 

@@ -1315,6 +1315,9 @@ int tg_int4_gemv_dequant(const int8_t* xq, const float* xscale, const uint8_t* w
 // ------------------------------------------------------------ routed experts
 namespace {
 
+// Most (token, expert) slots: 32-bit slot numbers, with room for a grid's stride.
+constexpr int64_t kMaxRouteSlots = int64_t(1) << 30;
+
 // Tokens per CTA of the router's two-kernel form, a multiple of 32: a warp a
 // token and 32 warps, more where that would make more than 256 CTAs, whose
 // counts every CTA of the second kernel reads.
@@ -1365,7 +1368,7 @@ int launch_combine(tg::CombineParams p, cudaStream_t st) {
 extern "C" {
 
 size_t tg_route_experts_workspace(int64_t T, int64_t E) {
-  if (T <= tg::route::SINGLE || E <= 0) return 0;
+  if (T <= tg::route::SINGLE || T > kMaxRouteSlots || E <= 0 || E > tg::route::MAX_E) return 0;
   const int per = route_per_block(T);
   return size_t((T + per - 1) / per) * size_t(E) * 4;
 }
@@ -1375,7 +1378,7 @@ int tg_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int to
                      size_t workspace_bytes, void* stream) {
   if (T < 0 || E <= 0 || top_k <= 0 || top_k > E || !is_dtype(dtype)) return TG_ERR_INVALID_ARG;
   if (E > tg::route::MAX_E || top_k > tg::route::MAX_K) return TG_ERR_UNSUPPORTED;
-  if (T > (int64_t(1) << 30) / top_k) return TG_ERR_UNSUPPORTED;  // 32-bit slot numbers, with room for a grid's stride
+  if (T > kMaxRouteSlots / top_k) return TG_ERR_UNSUPPORTED;
   if (!offsets || !aligned_to(offsets, 4)) return offsets ? TG_ERR_MISALIGNED : TG_ERR_INVALID_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0)
@@ -1454,6 +1457,12 @@ namespace {
 constexpr int64_t kGatherPassMinRows = 256;
 constexpr double kGatherPassMinWork = 1.25e11;
 
+// Sizes whose row numbers have 32 bits (E * N within 64 bits).
+bool grouped_in_range(int64_t R, int64_t E, int64_t N, int64_t K) {
+  return E <= tg::route::MAX_E && R <= kMaxTiledRows && K < (int64_t(1) << 31) && N <= kMaxTiledRows &&
+         E * N <= kMaxTiledRows;
+}
+
 // Rows an expert has on average, if every expert has some.
 int64_t grouped_avg(int64_t R, int64_t E) { return R / std::max<int64_t>(1, std::min(E, R)); }
 
@@ -1514,7 +1523,7 @@ int launch_grouped_tn(const int8_t* xq, const CUtensorMap& tw, const CUtensorMap
 extern "C" {
 
 size_t tg_int8_grouped_gemm_dequant_workspace(int64_t R, int64_t E, int64_t N, int64_t K) {
-  if (R <= 0 || E <= 0 || N <= 0 || K <= 0 || grouped_avg(R, E) < kGatherPassMinRows ||
+  if (R <= 0 || E <= 0 || N <= 0 || K <= 0 || !grouped_in_range(R, E, N, K) || grouped_avg(R, E) < kGatherPassMinRows ||
       double(R) * double(N) * double(K) < kGatherPassMinWork)
     return 0;
   return size_t(R) * size_t(K + 4);
@@ -1527,12 +1536,10 @@ int tg_int8_grouped_gemm_dequant(const int8_t* xq, const float* xscale, int64_t 
                                  void* stream) {
   if (M < 0 || R < 0 || E <= 0 || N <= 0 || K <= 0) return TG_ERR_INVALID_ARG;
   if (!is_dtype(out_dtype) || (bias && !is_dtype(bias_dtype))) return TG_ERR_INVALID_ARG;
-  if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
   if ((!rows && R > M) || (R > 0 && M == 0)) return TG_ERR_INVALID_ARG;
+  if (M > kMaxTiledRows || !grouped_in_range(R, E, N, K)) return TG_ERR_UNSUPPORTED;
+  if (wscale_numel != 1 && wscale_numel != E && wscale_numel != E * N) return TG_ERR_INVALID_ARG;
   if (K % 16 != 0 || (N * int64_t(dtype_bytes(out_dtype))) % 16 != 0) return TG_ERR_UNSUPPORTED;
-  if (E > tg::route::MAX_E || M > kMaxTiledRows || R > kMaxTiledRows || K >= (int64_t(1) << 31) ||
-      N > kMaxTiledRows || E * N > kMaxTiledRows)
-    return TG_ERR_UNSUPPORTED;
   if (R == 0) return TG_OK;
   if (!xq || !xscale || !wq || !wscale || !offsets || !out) return TG_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(wq) || !aligned16(out)) return TG_ERR_MISALIGNED;
