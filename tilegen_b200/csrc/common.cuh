@@ -105,20 +105,11 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait for the phase with the given parity to complete.  Returns false
-// (and ORs `err` into the device status) if it did not complete in time.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned int err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer_ns();
-  for (;;) {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      atomicOr(&g_device_status, err);
-      return false;
-    }
-  }
-}
+}  // namespace tg
+
+#include "waits.cuh"
+
+namespace tg {
 
 // ---------------------------------------------------------------- dequantisation
 // out = ((float(acc) * xs) * ws) + bias, one rounding per operation (no FMA),

@@ -264,10 +264,9 @@ __global__ void __launch_bounds__(gemv4::threads(WR), 1)
         }
       }
       // The loads in flight land before the CTA can exit or reuse the ring (after
-      // a wait gave up too).
-      for (int i = max(0, filled - p.stages); i < filled; ++i)
-        wait(&full_bar[i % p.stages], uint32_t(i / p.stages) & 1u, DEVERR_TMA_TIMEOUT);
-      wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT);
+      // a wait gave up too: these waits do not heed the flag).
+      ring_drain(full_bar, filled, p.stages, DEVERR_TMA_TIMEOUT);
+      mbar_wait(&scale_bar, 0u, DEVERR_TMA_TIMEOUT);
     }
   } else {
     if (scale_bulk != scale_len) {  // (the same for all warps)
