@@ -18,10 +18,10 @@ PROGRAM = r"""
 #define __forceinline__ inline
 namespace tg {
 constexpr unsigned long long kWaitLimitNs = 1000;
-unsigned long long g_clock = 0;
+unsigned long long g_clock = 0, g_tick = 0;
 unsigned int g_device_status = 0;
 void atomicOr(unsigned int* p, unsigned int v) { *p |= v; }
-unsigned long long globaltimer_ns() { return g_clock; }
+unsigned long long globaltimer_ns() { return g_clock += g_tick; }
 struct Poll { uint64_t bar; uint32_t parity; };
 std::vector<Poll> g_done;   // the waits that ended, in order
 int g_polls = 0;            // of the wait under way
@@ -56,6 +56,10 @@ int main() {
   const unsigned long long t0 = g_clock;
   ring_drain(bars, 9, 4, 4u);  // a load that never lands: its limit, then the others
   CHECK(g_device_status == 4 && g_done.size() == 3 && g_clock - t0 > kWaitLimitNs && g_clock - t0 < 2 * kWaitLimitNs);
+  const unsigned long long t1 = g_clock;
+  g_tick = 1;
+  wait_out();
+  CHECK(g_clock - t1 > kWaitLimitNs && g_clock - t1 < 2 * kWaitLimitNs);
   return 0;
 }
 """
@@ -79,3 +83,11 @@ def test_the_four_bit_kernel_drains_its_ring_with_them():
         text = f.read()
     tail = text[text.index("++filled"):text.index("named_barrier(1, WK * WR * 32)")]
     assert "ring_drain(full_bar, filled, p.stages" in tail and "mbar_wait(&scale_bar" in tail
+
+
+def test_the_grouped_kernel_leaves_nothing_in_flight():
+    """Once all roles of the CTA are done, not before: a flag that a slower role sets later would be missed."""
+    with open(os.path.join(_lib.CSRC_DIR, "gemm_grouped.cuh")) as f:
+        text = f.read()
+    tail = text[text.index("if (lane == 0) bulk_wait<0>();"):text.index("tmem_dealloc_pair(")]
+    assert tail.index("__syncthreads()") < tail.index("if (abort_flag && threadIdx.x == 0) wait_out()") < tail.index("cluster_sync()")

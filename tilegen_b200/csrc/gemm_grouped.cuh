@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
   __shared__ __align__(8) uint64_t tempty_bar[2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_flag;
-  __shared__ int issued;  // ring slots warp 0 filled
   __shared__ int cum[MAX_E + 1], start[MAX_E], count[MAX_E];
   __shared__ __align__(16) float col_xs[2][TN];
 
@@ -179,7 +178,6 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     }
     fence_mbar_init();
     abort_flag = 0;
-    issued = 0;
   }
   if (warp == 1) {
     tmem_alloc_pair(&tmem_base_sh, TMEM_COLS);
@@ -238,7 +236,7 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
     // activation rows in boxes.  Gathered ones are the other warps', so that the
     // weights' loads never wait for row numbers.
     static_assert(int(X_BYTES) / BK / 4 <= 32 * GATHERERS, "one gather per lane");
-    int stage = 0, n_issued = 0;
+    int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int t = unit; t < tiles && ok; t += units) {
@@ -290,14 +288,12 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
             tma_gather4_pair(sx + ks * X_BYTES + gr * BK, &tma_x, fb, (kb * KS + ks) * BK, idx);
         }
         __syncwarp();
-        ++n_issued;
         if (++stage == S) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    if (warp == 0 && lane == 0) issued = n_issued;
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && leader) {
@@ -409,13 +405,12 @@ __global__ void __launch_bounds__(grouped::threads(GATHER), 1)
   }
 
   __syncwarp();
-  // A wait gave up: let the loads still in flight (at most the last S slots)
-  // land before the CTA exits (they all land on the even CTA's barriers, and the
-  // odd one waits for it below).
-  if (abort_flag && threadIdx.x == 0 && leader) {
-    for (int i = max(0, issued - S); i < issued; ++i)
-      mbar_wait(&full_bar[i % S], uint32_t(i / S) & 1u, DEVERR_TMA_TIMEOUT);
-  }
+  // Every role is done; one that gave up has set the flag.  Loads (the odd CTA's land
+  // on the even one's barriers, a gather's perhaps on one that warp 0 did not announce)
+  // and products may then still be in flight.  A CTA whose roles all finished has
+  // none: its epilogue saw every product of the pair.
+  __syncthreads();
+  if (abort_flag && threadIdx.x == 0) wait_out();
   __syncwarp();
   tc_fence_before();
   // Neither CTA of a pair may leave while the other can still touch its shared

@@ -27,4 +27,13 @@ __device__ __forceinline__ void ring_drain(uint64_t* full_bar, int issued, int s
     mbar_wait(&full_bar[i % stages], uint32_t(i / stages) & 1u, err);
 }
 
+// Waits out the limit: what this CTA has in flight after a wait gave up has landed
+// by then, or never will.  For loads and products that complete on another CTA's
+// barriers, or on barriers that were not told of them.
+__device__ __forceinline__ void wait_out() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 <= kWaitLimitNs) {
+  }
+}
+
 }  // namespace tg
