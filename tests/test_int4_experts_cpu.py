@@ -142,6 +142,32 @@ def test_cpu_tensors_are_refused():
         ops.combine_experts(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
 
 
+def test_tangents_are_refused():
+    """A forward-mode dual input is refused as one that wants a gradient is, not stripped of its tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    x, up = torch.ones(2, 256), (torch.zeros(2, 512, 256, dtype=torch.int8), torch.zeros(2, 512), None)
+    down = (torch.zeros(2, 256, 512, dtype=torch.int8), torch.zeros(2, 256), None)
+    logits = torch.zeros(2, 2)
+    ops.no_gradient("f", x, None)
+    with fwd.dual_level():
+        ops.no_gradient("f", x, None)
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                with pytest.raises(ValueError, match="gradient"):
+                    ops.no_gradient("f", None, x, dual)
+                with pytest.raises(ValueError, match="gradient"):
+                    int4_linear(dual, torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(4, 2))
+                for args in ((dual, logits, None), (x, fwd.make_dual(logits, logits), None), (x, logits, dual)):
+                    with pytest.raises(ValueError, match="gradient"):
+                        int8_expert_ffn(args[0], args[1], up, down, 1, residual=args[2])
+    with torch.no_grad():
+        ops.no_gradient("f", x.clone().requires_grad_())
+    with pytest.raises(ValueError, match="gradient"):
+        ops.no_gradient("f", x.clone().requires_grad_())
+
+
 @pytest.mark.parametrize("e,n", [(3, 8), (1, 16), (2, 4)])
 def test_expert_scale_shapes(e, n):
     """A wscale of the right number of elements in the wrong order is refused."""

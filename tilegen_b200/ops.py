@@ -26,6 +26,7 @@ import contextlib
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -361,9 +362,14 @@ def _on(fn: str, name: str, t, dev: torch.device, dtypes, ndim: int) -> None:
 
 
 def no_gradient(fn: str, *tensors) -> None:
-    """The forms for serving have no backward pass: an input that wants a gradient is refused."""
+    """The forms for serving have no derivatives: an input that wants a gradient or carries a tangent is refused."""
+    wanted = torch.is_grad_enabled()
+    # Without a level of forward-mode differentiation (-1) no tensor has a tangent.
+    dual = getattr(forward_ad, "_current_level", 0) >= 0
+    if not (wanted or dual):
+        return
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is not None and (wanted and t.requires_grad or dual and forward_ad.unpack_dual(t).tangent is not None):
             raise ValueError(f"{fn}: no gradient is computed; call it under torch.no_grad() or on detached tensors")
 
 
