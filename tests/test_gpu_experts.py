@@ -345,6 +345,19 @@ def test_grouped_scale_shapes(cuda):
             ops.int8_grouped_gemm_dequant(xq, xs, wq, bad, bias, offsets, torch.float16, rows=rows)
 
 
+def test_deterministic_mode_fills_uncovered_rows(cuda):
+    """torch's deterministic mode fills new memory: rows that no group covers are NaN, not what was there before."""
+    xq, xs, wq, ws, bias, offsets, _ = _group_case([3, 4], 64, 128, seed=2)
+    offsets[-1] = 5
+    ref = ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, bias, offsets, torch.float16)
+    torch.use_deterministic_algorithms(True)
+    try:
+        y = ops.int8_grouped_gemm_dequant(xq, xs, wq, ws, bias, offsets, torch.float16)
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert torch.equal(y[:5], ref[:5]) and y[5:].isnan().all()
+
+
 # ---------------------------------------------------------------- combine
 def _check_combine(y, place, weights, residual, out=None):
     got = ops.combine_experts(y, place, weights, residual=None if residual is None else residual.clone(), out=out)

@@ -142,6 +142,39 @@ def test_cpu_tensors_are_refused():
         ops.combine_experts(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
 
 
+def test_allocations_do_not_pass_modes_by(monkeypatch):
+    """Outputs come from torch's own call where a dispatch mode or the deterministic fill has to see them, or the
+    device is not the current one."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        count = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Seen.count += 1
+            return func(*args, **(kwargs or {}))
+
+    fast, meta = [], torch.device("meta", 0)
+
+    def pretend(shape, stride, dtype):
+        fast.append(shape)
+        return torch.empty(shape, dtype=dtype)
+
+    monkeypatch.setattr(ops, "_fast_empty", pretend)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    ops._empty(meta, torch.float16, 3, 4)
+    assert fast == [(3, 4)]
+    with Seen():
+        assert ops._empty(meta, torch.float16, 3, 0).shape == (3, 0)
+    assert Seen.count == 1 and fast == [(3, 4)]
+    monkeypatch.setattr(torch, "are_deterministic_algorithms_enabled", lambda: True)
+    assert ops._empty(meta, torch.int32, 5).device.type == "meta" and len(fast) == 1
+    monkeypatch.undo()
+    monkeypatch.setattr(ops, "_fast_empty", pretend)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    assert ops._empty(meta, torch.int32, 5).device.type == "meta" and len(fast) == 1
+
+
 def test_tangents_are_refused():
     """A forward-mode dual input is refused as one that wants a gradient is, not stripped of its tangent."""
     import torch.autograd.forward_ad as fwd

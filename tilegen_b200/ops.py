@@ -71,15 +71,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 # the dispatcher's round (0.7 us where torch.empty takes 1.6), where torch has the
 # allocator entry that its own generated code uses.
 _fast_empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+# How many dispatch modes are active; without it (None) the dispatcher is not passed by.
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+
+
+def _allocator(dev: torch.device):
+    """(shape, stride, dtype) -> an uninitialised tensor on the CUDA device ``dev``: torch's own call on another device
+    than the current one, where a dispatch mode has to see it, and where the deterministic mode fills new memory."""
+    if (_fast_empty is not None and _dispatch_modes is not None and dev.index == torch.cuda.current_device()
+            and not _dispatch_modes() and not torch.are_deterministic_algorithms_enabled()):
+        return _fast_empty
+    return lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=dev)
 
 
 def _empty(dev: torch.device, dtype: torch.dtype, *shape: int) -> torch.Tensor:
     """``torch.empty`` of one or two dimensions on the CUDA device ``dev``."""
-    if _fast_empty is not None:
-        t = _fast_empty(shape, (1,) if len(shape) == 1 else (shape[1] or 1, 1), dtype)
-        if t.device == dev:
-            return t
-    return torch.empty(*shape, dtype=dtype, device=dev)
+    return _allocator(dev)(shape, (1,) if len(shape) == 1 else (shape[1] or 1, 1), dtype)
 
 
 def _call(func: str, dev: torch.device, *args) -> None:
@@ -474,8 +481,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True) ->
         raise ValueError(f"{fn}: {t} tokens of {top_k} experts are too many")
     no_gradient(fn, logits)
     logits = logits.contiguous()
-    empty = _fast_empty if _fast_empty is not None and dev.index == torch.cuda.current_device() else (
-        lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=dev))
+    empty = _allocator(dev)
     slots, stride, i32 = (t, top_k), (top_k, 1), torch.int32
     ids, place, weights = empty(slots, stride, i32), empty(slots, stride, i32), empty(slots, stride, torch.float32)
     offsets, rows = empty((e + 1,), (1,), i32), empty((t * top_k,), (1,), i32)
