@@ -228,6 +228,18 @@ def test_layer_functions_check_shapes():
         int8_expert_ffn(torch.zeros(3, 256), torch.zeros(3, 2), up, up, 1)
 
 
+def test_layer_checks_the_residuals_shape():
+    up = (torch.zeros(2, 512, 256, dtype=torch.int8), torch.zeros(2, 512), None)
+    down = (torch.zeros(2, 256, 512, dtype=torch.int8), torch.zeros(2, 256), None)
+    x, logits = torch.zeros(3, 4, 256), torch.zeros(3, 4, 2)
+    for shape in ((4, 3, 256), (3, 4, 255), (3, 256, 4), (1, 12, 256)):  # as many elements are not enough
+        with pytest.raises(ValueError, match="residual"):
+            int8_expert_ffn(x, logits, up, down, 1, residual=torch.zeros(shape))
+    for shape in ((3, 4, 256), (12, 256)):  # the next check is the device's
+        with pytest.raises(ValueError, match="CUDA"):
+            int8_expert_ffn(x, logits, up, down, 1, residual=torch.zeros(shape))
+
+
 @pytest.mark.parametrize("m", [1, 2, 63, 64, 65, 66, 127, 128, 129, 130, 193, 1025])
 def test_linear_leaves_no_single_row_behind(monkeypatch, m):
     """The blocks cover every row once, and only a one-row input goes to the one-row kernel, which adds in an order

@@ -30,7 +30,7 @@ def int8_expert_ffn(x: torch.Tensor, logits: torch.Tensor, up, down, top_k: int,
     ``x [..., K]`` fp16/bf16 on a CUDA device; ``logits [..., E]`` the router's; ``up``
     and ``down``: ``(wq, wscale, bias or None)`` with ``wq [E, F, K]`` and ``[E, K, F]`` int8
     rotated by ``group_size``; ``act`` None or a name in ``ops.FUSED_ACTS``, applied
-    in the second quantiser's pass; ``residual`` of ``x``'s shape and dtype.
+    in the second quantiser's pass; ``residual`` of ``x``'s shape (or its rows ``[T, K]``) and dtype.
     """
     k = x.shape[-1]
     x2 = x.reshape(-1, k)
@@ -38,6 +38,8 @@ def int8_expert_ffn(x: torch.Tensor, logits: torch.Tensor, up, down, top_k: int,
         raise ValueError(f"logits {tuple(logits.shape)} do not match x {tuple(x.shape)}")
     if down[0].shape[1] != k:
         raise ValueError(f"down projects to {down[0].shape[1]} channels, x has {k}")
+    if residual is not None and residual.shape not in (x.shape, x2.shape):
+        raise ValueError(f"residual {tuple(residual.shape)} is not of x's shape {tuple(x.shape)}")
     ops.no_gradient("int8_expert_ffn", x, logits, residual)
     routes = ops.route_experts(logits.reshape(-1, logits.shape[-1]), top_k, renormalize)
     xq, xscale = ops.rotate_quant(x2, group_size)
