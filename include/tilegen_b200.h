@@ -309,7 +309,8 @@ size_t tg_int8_grouped_gemm_dequant_workspace(int64_t R, int64_t E, int64_t N, i
  *
  *   y        [R, N] of dtype; place [T, top_k], a place outside [0, R) adds
  *            nothing; weights [T, top_k] fp32; residual [T, N] of dtype or NULL
- *   out      [T, N] of dtype (may be `residual` itself)
+ *   out      [T, N] of dtype (may be `residual` itself; TG_ERR_INVALID_ARG where
+ *            it shares memory with an input otherwise)
  * Any N; top_k <= TG_MAX_TOP_K.  T == 0 is a no-op.
  */
 int tg_combine_experts(const void *y, int dtype, int64_t R, const int32_t *place, const float *weights, int64_t T,

@@ -431,6 +431,22 @@ def test_combine_in_place_strides_and_refusals(cuda):
     assert ops.combine_experts(y, place[:0], w[:0]).shape == (0, 96)
 
 
+def test_combine_into_memory_of_an_input(cuda):
+    g = _gen(4)
+    whole = torch.randn(12, 96, generator=g, device=cuda)
+    y, res = whole[:8], whole[8:].clone()
+    place = torch.randint(0, 8, (4, 2), generator=g, dtype=torch.int32, device=cuda)
+    w = torch.rand(4, 2, generator=g, device=cuda)
+    for bad in (whole[:4], whole[4:8], whole[7:11]):
+        with pytest.raises(ValueError, match="invalid argument"):
+            ops.combine_experts(y, place, w, residual=res, out=bad)
+    pair = torch.cat([res, res])
+    with pytest.raises(ValueError, match="invalid argument"):
+        ops.combine_experts(y, place, w, residual=pair[1:5], out=pair[:4])
+    ref = ops.combine_experts(y, place, w, residual=res)
+    assert torch.equal(ops.combine_experts(y, place, w, residual=res, out=whole[8:]), ref)  # right behind y
+
+
 def test_combine_past_32_bit_offsets(cuda):
     y = torch.zeros(70000, 32768, dtype=torch.float16, device=cuda)
     y[-2:] = torch.randn(2, 32768, generator=_gen(5), device=cuda).half()

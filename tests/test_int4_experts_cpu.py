@@ -370,3 +370,20 @@ def _combine(y=P, dt=1, r=8, place=P, w=P, t=4, k=2, res=None, n=64, out=P):
 ])
 def test_combine_entry_checks(kwargs, status):
     assert _combine(**kwargs) == status
+
+
+@pytest.mark.parametrize("base,size", [("y", 8 * 64 * 2), ("place", 4 * 2 * 4), ("w", 4 * 2 * 4), ("res", 4 * 64 * 2)])
+def test_combine_refuses_an_out_that_overlaps_an_input(base, size):
+    """A fault of the call, not a race of its CTAs.  (What is in order gets as far as this machine's missing GPU, so
+    only the refusals are looked at.)"""
+    at = 1 << 20
+    buffers = {"y": at << 1, "place": at << 2, "w": at << 3, "res": at << 4}
+    pointers = {k: ctypes.c_void_p(v) for k, v in buffers.items()}
+    first, out_bytes = buffers[base], 4 * 64 * 2
+    for out in (first + 2, first + size - 2, first - out_bytes + 2) + (() if base == "res" else (first,)):
+        assert _combine(**pointers, out=ctypes.c_void_p(out)) == ARG
+    if torch.cuda.is_available():  # the others would be launched, on addresses that are not there
+        return
+    for out in (first + size, first - out_bytes) + ((first,) if base == "res" else ()):
+        assert _combine(**pointers, out=ctypes.c_void_p(out)) != ARG
+    assert _combine(**{**pointers, "y": None}, r=0, out=ctypes.c_void_p(1 << 26)) != ARG

@@ -1080,6 +1080,12 @@ size_t dtype_bytes(int d) { return d == TG_DT_F32 ? 4 : 2; }
 
 bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Whether two buffers share a byte.
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x <= y ? y - x < a_bytes : x - y < b_bytes;
+}
+
 // A launch as the programmatic dependent of the kernel before it.
 template <typename P>
 int launch_dependent(void (*kern)(const P), const P& p, dim3 grid, int threads, uint32_t smem, cudaStream_t st) {
@@ -1426,6 +1432,12 @@ int tg_combine_experts(const void* y, int dtype, int64_t R, const int32_t* place
   if (!aligned_to(y, esz) || !aligned_to(out, esz) || !aligned_to(residual, esz) || !aligned_to(place, 4) ||
       !aligned_to(weights, 4))
     return TG_ERR_MISALIGNED;
+  // A row of out is written while others are still to be read.
+  const uint64_t out_bytes = uint64_t(T) * uint64_t(N) * esz, slot_bytes = uint64_t(T) * uint64_t(top_k) * 4u;
+  if ((R > 0 && overlap(out, out_bytes, y, uint64_t(R) * uint64_t(N) * esz)) ||
+      (residual && residual != out && overlap(out, out_bytes, residual, out_bytes)) ||
+      overlap(out, out_bytes, place, slot_bytes) || overlap(out, out_bytes, weights, slot_bytes))
+    return TG_ERR_INVALID_ARG;
   tg::CombineParams p;
   p.y = y;
   p.place = place;

@@ -573,7 +573,8 @@ def combine_experts(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor,
     ``y [R, N]`` fp32/fp16/bf16; ``place [T, k]`` int32 and ``weights [T, k]`` fp32 as
     ``route_experts`` returns them (a place outside ``[0, R)`` adds nothing);
     ``residual [T, N]`` of ``y``'s dtype or None.  ``out``: an optional contiguous ``[T,
-    N]`` tensor to write into, which may be ``residual`` itself.
+    N]`` tensor to write into, which may be ``residual`` itself but shares no memory
+    with an input otherwise.
     """
     fn = "combine_experts"
     if not isinstance(y, torch.Tensor) or not y.is_cuda:
