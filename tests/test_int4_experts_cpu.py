@@ -161,18 +161,23 @@ def test_allocations_do_not_pass_modes_by(monkeypatch):
         return torch.empty(shape, dtype=dtype)
 
     monkeypatch.setattr(ops, "_fast_empty", pretend)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    ops._empty(meta, torch.float16, 3, 4)
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+
+    def alloc(*shape):
+        return ops._out("f", None, shape, torch.float16, meta)
+
+    alloc(3, 4)
     assert fast == [(3, 4)]
     with Seen():
-        assert ops._empty(meta, torch.float16, 3, 0).shape == (3, 0)
+        assert alloc(3, 0).shape == (3, 0)
     assert Seen.count == 1 and fast == [(3, 4)]
-    monkeypatch.setattr(torch, "are_deterministic_algorithms_enabled", lambda: True)
-    assert ops._empty(meta, torch.int32, 5).device.type == "meta" and len(fast) == 1
-    monkeypatch.undo()
-    monkeypatch.setattr(ops, "_fast_empty", pretend)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
-    assert ops._empty(meta, torch.int32, 5).device.type == "meta" and len(fast) == 1
+    torch.use_deterministic_algorithms(True)
+    try:
+        assert alloc(5, 2).device.type == "meta" and len(fast) == 1
+    finally:
+        torch.use_deterministic_algorithms(False)
+    monkeypatch.setattr(ops, "_current_device", lambda: 1)
+    assert alloc(5, 2).device.type == "meta" and len(fast) == 1
 
 
 def test_tangents_are_refused():

@@ -73,25 +73,23 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _fast_empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 # How many dispatch modes are active; without it (None) the dispatcher is not passed by.
 _dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_deterministic = getattr(torch._C, "_get_deterministic_algorithms", torch.are_deterministic_algorithms_enabled)
+# The current device once CUDA is in use, which an input on a CUDA device shows.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _allocator(dev: torch.device):
     """(shape, stride, dtype) -> an uninitialised tensor on the CUDA device ``dev``: torch's own call on another device
     than the current one, where a dispatch mode has to see it, and where the deterministic mode fills new memory."""
-    if (_fast_empty is not None and _dispatch_modes is not None and dev.index == torch.cuda.current_device()
-            and not _dispatch_modes() and not torch.are_deterministic_algorithms_enabled()):
+    if (_fast_empty is not None and _dispatch_modes is not None and dev.index == _current_device()
+            and not _dispatch_modes() and not _deterministic()):
         return _fast_empty
     return lambda shape, stride, dtype: torch.empty_strided(shape, stride, dtype=dtype, device=dev)
 
 
-def _empty(dev: torch.device, dtype: torch.dtype, *shape: int) -> torch.Tensor:
-    """``torch.empty`` of one or two dimensions on the CUDA device ``dev``."""
-    return _allocator(dev)(shape, (1,) if len(shape) == 1 else (shape[1] or 1, 1), dtype)
-
-
 def _call(func: str, dev: torch.device, *args) -> None:
     L = _lib.lib()
-    current = torch.cuda.current_device()
+    current = _current_device()
     idx = dev.index if dev.index is not None else current
     stream = _raw_stream(idx)
     if idx != current:
@@ -368,11 +366,14 @@ def _on(fn: str, name: str, t, dev: torch.device, dtypes, ndim: int) -> None:
     raise ValueError(f"{fn}: {name} must be {ndim}-D of {' / '.join(map(str, dtypes))}, got {tuple(t.shape)} {t.dtype}")
 
 
+# The level of forward-mode differentiation: without one (-1) no tensor has a tangent.
+_dual_level = (lambda: forward_ad._current_level) if hasattr(forward_ad, "_current_level") else (lambda: 0)
+
+
 def no_gradient(fn: str, *tensors) -> None:
     """The forms for serving have no derivatives: an input that wants a gradient or carries a tangent is refused."""
     wanted = torch.is_grad_enabled()
-    # Without a level of forward-mode differentiation (-1) no tensor has a tangent.
-    dual = getattr(forward_ad, "_current_level", 0) >= 0
+    dual = _dual_level() >= 0
     if not (wanted or dual):
         return
     for t in tensors:
@@ -380,10 +381,10 @@ def no_gradient(fn: str, *tensors) -> None:
             raise ValueError(f"{fn}: no gradient is computed; call it under torch.no_grad() or on detached tensors")
 
 
-def _out(fn: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, dev: torch.device,
+def _out(fn: str, out: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype, dev: torch.device,
          align: int = 16) -> torch.Tensor:
     if out is None:
-        return _empty(dev, dtype, *shape)
+        return _allocator(dev)(shape, (shape[1] or 1, 1), dtype)
     if (tuple(out.shape) != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous()
             or out.data_ptr() % align):
         raise ValueError(f"{fn}: out must be a contiguous {align}-byte aligned {list(shape)} {dtype} tensor on {dev}")
@@ -558,7 +559,7 @@ def int8_grouped_gemm_dequant(xq: torch.Tensor, xscale: torch.Tensor, wq: torch.
     out = _out(fn, out, (r, n), out_dtype, dev)
     if r:
         need = 0 if rows is None else _lib.lib().tg_int8_grouped_gemm_dequant_workspace(r, e, n, k)
-        work = _empty(dev, torch.uint8, need) if need else None
+        work = _allocator(dev)((need,), (1,), torch.uint8) if need else None
         _call("tg_int8_grouped_gemm_dequant", dev, xq.data_ptr(), xscale.data_ptr(), m, wq.data_ptr(),
               wscale.data_ptr(), wscale.numel(), b_ptr, b_code, r_ptr, offsets.data_ptr(), r, e, n, k,
               _DTYPE_CODE[out_dtype], out.data_ptr(), work.data_ptr() if need else None, need)
