@@ -571,6 +571,41 @@ def test_layers_on_two_streams_at_once(cuda):
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+def test_first_calls_from_many_threads_at_once(cuda):
+    """A fresh process whose first calls come from eight threads together, each on a stream of its own."""
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+from tilegen_b200 import ops
+from tilegen_b200.quant import pack_int4
+g = torch.Generator(device="cuda").manual_seed(1)
+xq = torch.randint(-128, 128, (12, 512), generator=g, dtype=torch.int8, device="cuda")
+codes = torch.randint(-8, 8, (96, 512), generator=g, dtype=torch.int8, device="cuda")
+xs, ws = torch.rand(12, generator=g, device="cuda"), torch.rand(96, 4, generator=g, device="cuda")
+wq, w4 = torch.randint(-128, 128, (2, 64, 512), generator=g, dtype=torch.int8, device="cuda"), pack_int4(codes)
+logits, one = torch.randn(12, 2, generator=g, device="cuda"), torch.ones(1, device="cuda")
+torch.cuda.synchronize()
+start, out = threading.Barrier(8), [None] * 8
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        a = [ops.int4_gemv_dequant(xq[:m], xs[:m], w4, ws, None, torch.float32) for m in (1, 12)]
+        r = ops.route_experts(logits, 1)
+        y = ops.int8_grouped_gemm_dequant(xq, xs, wq, one, None, r.offsets, torch.float32, rows=r.rows)
+        out[i] = (*a, *r, y, ops.combine_experts(y, r.place, r.weights))
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for i in range(8):
+    assert all(torch.equal(p, q) for p, q in zip(out[i], out[0])), i
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, f"{done.returncode}: {done.stderr[-800:]}"
+
+
 def test_grouped_with_few_sms(cuda):
     """The SM budget's smallest grids still cover every tile."""
     case = _group_case([300, 0, 5, 40], 520, 512, 60, seed=3)

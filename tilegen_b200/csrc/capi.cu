@@ -50,15 +50,14 @@ struct DeviceInfo {
 std::atomic<int> g_sm_budget{0};
 
 bool current_device(int* dev, DeviceInfo* info) {
-  static DeviceInfo cache[kMaxDevices];
+  static std::atomic<int> known[kMaxDevices];  // SMs; 0: not asked yet.  Threads may make their first calls together.
   if (cudaGetDevice(dev) != cudaSuccess || *dev < 0 || *dev >= kMaxDevices) return false;
-  if (cache[*dev].sms == 0) {
-    int v = 0;
-    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess) return false;
-    cache[*dev].sms = v;
-    cache[*dev].sms_all = v;
+  int v = known[*dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess || v <= 0) return false;
+    known[*dev].store(v, std::memory_order_relaxed);
   }
-  *info = cache[*dev];
+  info->sms = info->sms_all = v;
   const int budget = g_sm_budget.load(std::memory_order_relaxed);
   if (budget > 0 && budget < info->sms) info->sms = budget;
   return true;
