@@ -224,10 +224,11 @@ int tg_int8_gemv_dequant_config(int64_t N, int64_t K, int *parts, int *ctas);
  *
  *   out[m,n] = (sum_g wscale[n,g] * float(sum_{k in g} xq[m,k] * w4[n,k])) * xscale[m] + bias[n]
  *
- * The inner sums are exact (a group of 256: each half's), the outer one is fp32
- * in an order of its own for M == 1 (a kernel for one row) and in one that
- * depends on K only from M == 2 up: there a row's result depends neither on the
- * other rows nor on M.
+ * From M == 2 up the inner sums are exact (a group of 256: each half's) and the
+ * outer one is fp32 in an order that depends on K only: a row's result depends
+ * neither on the other rows nor on M.  M == 1 has a kernel of its own: the sums
+ * over 8, 16 or 32 codes of a group (of 32, 64, more) are exact, and these are
+ * added in fp32 in another order.
  *
  *   xq      [M, K] int8, 16-B aligned; K % 128 == 0, K at most
  *           tg_rotate_quant_max_k()

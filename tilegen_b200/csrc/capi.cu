@@ -1140,7 +1140,7 @@ static_assert(gemv4_always_fits(1, 1) && gemv4_always_fits(1, 2) && gemv4_always
               gemv4_always_fits(4, 1) && gemv4_always_fits(8, 1), "a form for every size");
 
 // K parts per group of four weight rows, as gemv_parts: the fewest that put two
-// CTAs on every SM, each part keeping two chunks a lane.
+// CTAs on every SM, each part keeping at least one 16-byte chunk a lane.
 int gemv4_parts(int64_t N, int64_t K, int sms) {
   using namespace tg::gemv4one;
   const int64_t row_groups = (N + R - 1) / R, nch = K / 32;
@@ -1160,7 +1160,7 @@ int launch_gemv4_one_t(const tg::GemvI4OneParams& p, int64_t ctas, cudaStream_t 
 // SM, and help where the launch is one wave of those and a lane has more than two
 // chunks; otherwise four CTAs per SM with one chunk each carry more.  Measured (K x
 // N, two / one, us): 13824 x 5120 8.6 / 9.6, 5120 x 5120 5.2 / 5.35; 5120 x 15360
-// (480 CTAs) 11.4 / 8.0, 2048 x 1536 (two chunks a lane) 2.3 / 2.15.  Groups of 32
+// (480 CTAs) 11.4 / 8.0, 2048 x 1536 (one chunk a lane) 2.3 / 2.15.  Groups of 32
 // with fp32 scales are 16 more registers a chunk and spilled: 12.7 / 11.2.
 template <int SV, bool S4>
 int launch_gemv4_one_sv(const tg::GemvI4OneParams& p, int sms, cudaStream_t st) {

@@ -20,7 +20,11 @@
 // before it, and no atomic's order decides anything.  Up to SINGLE tokens one CTA
 // does everything; above, a first kernel writes the choices and each CTA's
 // counts, a second one adds up the counts of the CTAs before it and places the
-// slots.  The launches and a few dependent memory latencies bound it.  Neither of
+// slots.  Measured (us, top 8 of 64 / 256 / 1024 experts): one CTA, 1 token 2.9 / 4.0
+// / 9.2, 32 tokens 4.0 / 7.4 / 20.5, 64 6.3 / 12.2 / 34.8, 256 20.2 / 40.7 / 117; two
+// kernels, 257 tokens 5.9 / 9.3 / 23.3: the one CTA is the faster up to about 32 to 60
+// tokens, and one launch up to SINGLE.  The launches and a few dependent memory
+// latencies bound the two kernels, one SM's issue rate the one CTA.  Neither of
 // the two lets the kernel after it start early: CTAs that wait on SMs which are
 // done first leave the later ones unevenly placed (4096 tokens: 12.9 us, not 9.2).
 #pragma once
@@ -447,7 +451,9 @@ struct CombineParams {
 // VEC elements of a row per thread (16 bytes, or one where a row or an address
 // is not a multiple of 16 bytes).  One pass over the rows, HBM bound: a thread's
 // residual and two slots' loads are in flight together, and 42 registers keep six
-// CTAs of 256 threads on an SM.
+// CTAs of 256 threads on an SM.  4096 tokens, top 2, fp32 / 16-bit: 73 / 34 us at N =
+// 5120 (the bytes: 51 / 26), 121 / 166 at N = 5119, where one element a thread keeps
+// too few bytes in flight.
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256, 6) combine_kernel(const CombineParams p) {
   constexpr int ESZ = DT == TG_DT_F32 ? 4 : 2;

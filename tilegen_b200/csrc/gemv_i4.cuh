@@ -6,6 +6,7 @@
 // xq are the quantiser's int8 codes, w4 signed 4-bit codes (-8..7), g runs over
 // groups of 32, 64, 128 or 256 consecutive input channels.  The sum over a group
 // (each half of a group of 256) is exact (int32); these sums are added in fp32.
+// (With one row: the sums over a group's 8, 16 or 32 codes in 16 bytes of weight.)
 //
 // Weight layout (K a multiple of 128; K/2 bytes a row): of each block of 128
 // codes, byte 16 t + 4 j + b (t, j, b in 0..3) holds code 32 j + 8 t + b in its
@@ -18,10 +19,12 @@
 //
 // What bounds it: the weight's bytes, while the rows are few.  The weight comes
 // through a ring of shared memory by TMA, which keeps tens of KB in flight per SM
-// without a register, and is the products' M operand (legacy mma.sync: at 64 rows
-// the products are 20 % of its measured 1140 TOP/s at the weight's HBM rate, and
-// tcgen05 would need the unpacked weight written back to shared memory); the
-// activations are the N operand, 8 rows a product.
+// without a register, and is the products' M operand; the activations are the N
+// operand, 8 rows a product.  Legacy mma.sync, because tcgen05 needs the unpacked
+// weight written back to shared memory: at the weight's HBM rate 16 rows take 420 of
+// its measured 1140 TOP/s, 44 rows all of them and 64 rows 1680, so that from there
+// on the products are the floor (64 x 5120 x 15360: 8.8 us, the bytes 6.2).  33 rows
+// pay for 64 columns, 17 for 32, 9 for 16.
 //  * A CTA has WR * RT * 16 weight rows and all of K.  A step is one or two blocks
 //    of 128 codes for each of the four warps along K, so the activations of a
 //    step are read once per CTA.  The order of all additions depends on K alone: a
