@@ -91,3 +91,10 @@ def test_the_grouped_kernel_leaves_nothing_in_flight():
         text = f.read()
     tail = text[text.index("if (lane == 0) bulk_wait<0>();"):text.index("tmem_dealloc_pair(")]
     assert tail.index("__syncthreads()") < tail.index("if (abort_flag && threadIdx.x == 0) wait_out()") < tail.index("cluster_sync()")
+
+
+def test_the_tiled_kernel_leaves_nothing_in_flight():
+    with open(os.path.join(_lib.CSRC_DIR, "gemm_i8.cuh")) as f:
+        text = f.read()
+    tail = text[text.index("\ndone:"):text.index("tmem_dealloc_pair(tmem_base")]
+    assert tail.index("__syncthreads()") < tail.index("if (abort_flag && threadIdx.x == 0) wait_out()") < tail.index("cluster_sync()")

@@ -447,6 +447,11 @@ __global__ void __launch_bounds__(gemm::THREADS, 1)
 
 done:
   __syncwarp();
+  // Every role is done; one that gave up has set the flag.  Its loads (a pair's land on
+  // the even CTA's barriers) and products may then still be in flight.
+  __syncthreads();
+  if (abort_flag && threadIdx.x == 0) wait_out();
+  __syncwarp();
   tc_fence_before();
   // Neither CTA of a pair may leave while the other can still touch its
   // shared memory or tensor memory.
